@@ -35,7 +35,7 @@ enum {
   B200CONV_E_NCCL = -6
 };
 
-enum { B200CONV_F32 = 0, B200CONV_F16 = 1 };
+enum { B200CONV_F32 = 0, B200CONV_F16 = 1, B200CONV_BF16 = 2 /* the sequence operators only */ };
 
 /* Flags (bitwise or). */
 enum {
@@ -218,6 +218,69 @@ int b200conv_elementwise(b200conv_ctx* ctx, int op, const void* a, const void* b
 /* out[c] = sum over the pixels of x[pixel][c]: C values of the tensor dtype in device memory,
  * accumulated in float32 in a fixed order. */
 int b200conv_channel_sum(b200conv_ctx* ctx, const void* x, void* out, long long pixels, int C, int dtype);
+
+/* ---- sequence operators ---------------------------------------------------------------- */
+/* Layers of sequence models beside the convolutions: layer norm, the short causal convolution of every channel with
+ * its own filter (the reference runs causal convolutions through the 2-D path,
+ * theano/tensor/nnet/abstract_conv.py, causal_conv1d) and the selective state space scan (the reference leaves
+ * recurrences to its scan op).  Tensors are rows of channels in device memory, [sequences][length][C] with the channels
+ * contiguous and any distance between rows, in float32, float16 or bfloat16; sums and states are float32.  A
+ * channels-last image tensor is such a tensor with H * W rows per image and b200conv_padded_channels() elements per row.
+ *
+ * b200conv_rows says how one tensor lies in memory, in elements: from a row to the next and from a sequence's first row
+ * to the next sequence's.  `stored` (outputs): a row's channels C .. stored - 1 are written as zeros, which is what the
+ * pad channels of a channels-last image must hold; 0 or C writes nothing beyond C.
+ *
+ * An output may be an input of the same shape and strides where a call says so; otherwise outputs overlap neither inputs nor
+ * each other (rows of two tensors may interleave: halves of one wider tensor are fine).  The calls are asynchronous, run on
+ * the context's stream, allocate their workspace from its pool and can be captured into a graph, which keeps its own.
+ * Results do not depend on timing: every sum has a fixed order. */
+typedef struct b200conv_rows {
+  int64_t row, seq;
+  int32_t stored, reserved;
+} b200conv_rows;
+
+/* Layer norm over the C channels of sequences * length rows.
+ *   t = x + residual (rounded to the tensors' type), y = (t - mean) * rstd * gamma + beta, rstd = 1 / sqrt(var + eps)
+ * residual, gamma, beta, total and stats may be NULL.  total receives t (it may be x or residual; y may be x too), stats
+ * (mean, rstd) per row as float32 pairs.  gamma and beta hold C values of the tensors' type, or float32 with param_f32.
+ * The gradient takes t as x, and stats as the forward call left them:
+ *   dx = rstd * (g - mean(g) - hat * mean(g * hat)) + dtotal, g = dy * gamma, hat = (x - mean) * rstd
+ * dx may be dy or dtotal; dtotal (the gradient that reaches t on other ways), dgamma and dbeta may be NULL. */
+typedef struct b200conv_norm_desc {
+  int64_t sequences, length;
+  int32_t C, dtype, param_f32;
+  float eps;
+  b200conv_rows x, residual, y, total, dy, dtotal, dx;
+} b200conv_norm_desc;
+int b200conv_layer_norm(b200conv_ctx* ctx, const b200conv_norm_desc* d, const void* x, const void* residual,
+                        const void* gamma, const void* beta, void* y, void* total, float* stats);
+int b200conv_layer_norm_grad(b200conv_ctx* ctx, const b200conv_norm_desc* d, const void* dy, const void* x,
+                             const void* gamma, const float* stats, const void* dtotal, void* dx, void* dgamma, void* dbeta);
+
+/* Short causal convolution: every channel with its own filter of 2 to 8 taps.
+ *   pre[t][c] = bias[c] + sum over k of w[c][k] * x[t - k][c]   (flip; without it w[c][width - 1 - k]),
+ *   y = silu ? pre * sigmoid(pre) : pre
+ * w is [C][width], bias (may be NULL) C values, both of the tensors' type or float32 with param_f32.  The rows before a
+ * sequence's first token come from `initial`, [sequences][width - 1][C] in the tensors' type, oldest first; NULL: zeros.
+ * `final` (may be NULL, may be `initial`) receives the same for what follows: the last width - 1 rows of (initial, x).
+ * Packed sequences (`packed`): the tensors have `length` rows, sequence i takes rows starts[i] to starts[i + 1] - 1, with
+ * sequences + 1 offsets in device memory that do not decrease and do not exceed length; sequences may be empty, rows of no
+ * sequence are neither read nor written.  Offsets that break this give wrong results, no access outside of the tensors.
+ * The gradient: dx, and where given dw and dbias (like w, bias) and dinitial (like initial).
+ * The step takes one token of every sequence ([sequences][C]: length 1) and moves `state`, like initial, on in place. */
+typedef struct b200conv_causal_desc {
+  int64_t sequences, length;
+  int32_t C, width, dtype, param_f32, flip, silu, packed, reserved;
+  b200conv_rows x, y, dy, dx;
+} b200conv_causal_desc;
+int b200conv_causal_conv(b200conv_ctx* ctx, const b200conv_causal_desc* d, const void* x, const void* w, const void* bias,
+                         const void* initial, const int32_t* starts, void* y, void* final);
+int b200conv_causal_conv_grad(b200conv_ctx* ctx, const b200conv_causal_desc* d, const void* dy, const void* x, const void* w,
+                              const void* bias, const void* initial, const int32_t* starts, void* dx, void* dw, void* dbias,
+                              void* dinitial);
+int b200conv_causal_conv_step(b200conv_ctx* ctx, const b200conv_causal_desc* d, const void* x, const void* w,
+                              const void* bias, void* state, void* y);
 
 /* ---- device-resident tensors -------------------------------------------------------- */
 /* Channel count of the channels-last device layout (rounded up to 16 bytes). */

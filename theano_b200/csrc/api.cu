@@ -18,6 +18,7 @@
 #include <vector>
 
 #include "internal.h"
+#include "sequence.h"
 #include "staging.h"
 
 using namespace b200;
@@ -189,9 +190,9 @@ int fail(b200conv_ctx* c, int code, const char* fmt, ...) {
   } while (0)
 
 // Kernel families, for the launch counter and the optional per-kernel timing.
-enum { kKConvUmma = 0, kKWgradUmma, kKWgradReduce, kKTranspose, kKPack, kKDirect, kKPool, kKConvReduce, kKCount };
+enum { kKConvUmma = 0, kKWgradUmma, kKWgradReduce, kKTranspose, kKPack, kKDirect, kKPool, kKConvReduce, kKNorm, kKCausal, kKCount };
 const char* const kKernelNames[kKCount] = {"conv_umma", "wgrad_umma", "wgrad_reduce", "transpose",
-                                           "pack", "direct", "pool", "conv_reduce"};
+                                           "pack", "direct", "pool", "conv_reduce", "layer_norm", "causal_conv"};
 
 cudaEvent_t prof_event(b200conv_ctx* c) {
   cudaEvent_t e = nullptr;
@@ -221,6 +222,12 @@ cudaEvent_t prof_event(b200conv_ctx* c) {
       (c)->prof_recs.push_back({kind, ea_, eb_});               \
     }                                                           \
   } while (0)
+
+// Launches of an entry point that makes several, beyond the one that KLAUNCH counts.
+void count_launches(b200conv_ctx* c, int n) {
+  c->launches += n;
+  if (c->capturing) c->capturing->launches += n;
+}
 
 struct DeviceGuard {
   int prev = -1;
@@ -3365,6 +3372,181 @@ int b200conv_channel_sum(b200conv_ctx* c, const void* x, void* out, long long pi
   int rc = tmp.get(sizeof(float) * Cp * channel_sum_blocks(pixels), reinterpret_cast<void**>(&partial));
   if (rc) return rc;
   KLAUNCH(c, kKTranspose, launch_channel_sum(x, partial, out, pixels, C, Cp, dtype, c->stream));
+  return 0;
+}
+
+// ---- sequence operators -------------------------------------------------------------------
+// Checks that they share: types, sizes and strides.  Pointers to device memory cannot be looked into.
+static int check_rows(b200conv_ctx* c, const char* name, const void* p, const b200conv_rows& r, long long sequences, long long length, int C,
+                      bool written = false) {
+  if (!p || sequences * length == 0) return 0;
+  if (r.stored < 0 || r.row < 0 || r.seq < 0) return fail(c, B200CONV_E_INVALID, "%s: negative stride", name);
+  const long long stored = std::max(C, r.stored);
+  if (written && ((length > 1 && r.row < stored) || (sequences > 1 && r.seq < stored)))
+    return fail(c, B200CONV_E_INVALID, "%s: rows of %lld channels overlap (%lld elements between rows, %lld between sequences)", name, stored,
+                (long long)r.row, (long long)r.seq);
+  return 0;
+}
+static int check_sizes(b200conv_ctx* c, long long sequences, long long length, long long C, int dtype) {
+  if (dtype != B200CONV_F32 && dtype != B200CONV_F16 && dtype != B200CONV_BF16)
+    return fail(c, B200CONV_E_INVALID, "dtype must be float32, float16 or bfloat16");
+  if (sequences < 0 || length < 0 || C < 0) return fail(c, B200CONV_E_INVALID, "negative dimension");
+  if (sequences > INT32_MAX || length > INT32_MAX || sequences * length > INT32_MAX)
+    return fail(c, B200CONV_E_UNSUPPORTED, "more than 2^31 - 1 rows (%lld sequences of %lld)", sequences, length);
+  return 0;
+}
+
+int b200conv_layer_norm(b200conv_ctx* c, const b200conv_norm_desc* d, const void* x, const void* residual, const void* gamma, const void* beta,
+                        void* y, void* total, float* stats) {
+  if (!c) return B200CONV_E_INVALID;
+  std::lock_guard<std::mutex> g(c->mu);
+  DeviceGuard dg(c->device);
+  if (!d) return fail(c, B200CONV_E_INVALID, "null descriptor");
+  int rc = check_sizes(c, d->sequences, d->length, d->C, d->dtype);
+  if (rc) return rc;
+  if (d->C == 0) return fail(c, B200CONV_E_INVALID, "layer norm over no channels");
+  if (!(d->eps >= 0.f)) return fail(c, B200CONV_E_INVALID, "eps must not be negative");
+  if (d->sequences * d->length == 0) return 0;
+  if (!x || !y) return fail(c, B200CONV_E_INVALID, "layer norm without input or output");
+  if ((rc = check_rows(c, "x", x, d->x, d->sequences, d->length, d->C)) || (rc = check_rows(c, "residual", residual, d->residual, d->sequences, d->length, d->C)) ||
+      (rc = check_rows(c, "y", y, d->y, d->sequences, d->length, d->C, true)) || (rc = check_rows(c, "total", total, d->total, d->sequences, d->length, d->C, true)))
+    return rc;
+  NormArgs a = {};
+  a.d = *d;
+  a.x = x; a.residual = residual; a.gamma = gamma; a.beta = beta; a.y = y; a.total = total; a.stats = stats;
+  KLAUNCH(c, kKNorm, launch_layer_norm(a, c->stream));
+  return 0;
+}
+
+int b200conv_layer_norm_grad(b200conv_ctx* c, const b200conv_norm_desc* d, const void* dy, const void* x, const void* gamma, const float* stats,
+                             const void* dtotal, void* dx, void* dgamma, void* dbeta) {
+  if (!c) return B200CONV_E_INVALID;
+  std::lock_guard<std::mutex> g(c->mu);
+  DeviceGuard dg(c->device);
+  if (!d) return fail(c, B200CONV_E_INVALID, "null descriptor");
+  int rc = check_sizes(c, d->sequences, d->length, d->C, d->dtype);
+  if (rc) return rc;
+  if (d->C == 0) return fail(c, B200CONV_E_INVALID, "layer norm over no channels");
+  const size_t pbytes = (d->param_f32 ? 4 : row_elem_size(d->dtype)) * static_cast<size_t>(d->C);
+  if (d->sequences * d->length == 0) {              // sums over no rows
+    if (dgamma) CU_OK(c, cudaMemsetAsync(dgamma, 0, pbytes, c->stream));
+    if (dbeta) CU_OK(c, cudaMemsetAsync(dbeta, 0, pbytes, c->stream));
+    return 0;
+  }
+  if (!x || !dy || !stats || !dx) return fail(c, B200CONV_E_INVALID, "layer norm gradient without dy, x, stats or dx");
+  if ((rc = check_rows(c, "x", x, d->x, d->sequences, d->length, d->C)) || (rc = check_rows(c, "dy", dy, d->dy, d->sequences, d->length, d->C)) ||
+      (rc = check_rows(c, "dtotal", dtotal, d->dtotal, d->sequences, d->length, d->C)) || (rc = check_rows(c, "dx", dx, d->dx, d->sequences, d->length, d->C, true)))
+    return rc;
+  Scratch tmp(c);
+  NormArgs a = {};
+  a.d = *d;
+  a.x = x; a.gamma = gamma; a.dy = dy; a.dtotal = dtotal; a.dx = dx; a.dgamma = dgamma; a.dbeta = dbeta;
+  a.stats = const_cast<float*>(stats);
+  if ((dgamma || dbeta) &&
+      (rc = tmp.get(sizeof(float) * 2 * d->C * static_cast<size_t>(norm_grad_parts(*d)), reinterpret_cast<void**>(&a.partial))))
+    return rc;
+  int launches = 0;
+  KLAUNCH(c, kKNorm, launch_layer_norm_grad(a, &launches, c->stream));
+  count_launches(c, launches - 1);
+  return 0;
+}
+
+// Whether two arrays of `bytes` share memory (a state that is moved on in place).
+static bool overlap(const void* a, const void* b, size_t bytes) {
+  const char *p = static_cast<const char*>(a), *q = static_cast<const char*>(b);
+  return p && q && p < q + bytes && q < p + bytes;
+}
+// `initial`, or a copy of it where the call writes the final states over it: blocks of one launch read the one and write the other.
+static int detach_state(b200conv_ctx* c, Scratch& tmp, const void** initial, const void* final, size_t bytes) {
+  if (!bytes || !overlap(*initial, final, bytes)) return 0;
+  void* copy = nullptr;
+  int rc = tmp.get(bytes, &copy);
+  if (rc) return rc;
+  CU_OK(c, cudaMemcpyAsync(copy, *initial, bytes, cudaMemcpyDeviceToDevice, c->stream));
+  *initial = copy;
+  return 0;
+}
+
+static int check_causal(b200conv_ctx* c, const b200conv_causal_desc* d, const void* x, const void* w, const int32_t* starts) {
+  if (!d) return fail(c, B200CONV_E_INVALID, "null descriptor");
+  int rc = check_sizes(c, d->packed ? 1 : d->sequences, d->length, d->C, d->dtype);
+  if (rc) return rc;
+  if (d->sequences < 0 || d->sequences > INT32_MAX / 8) return fail(c, B200CONV_E_INVALID, "%lld sequences", (long long)d->sequences);
+  if (d->width < 2 || d->width > 8) return fail(c, B200CONV_E_UNSUPPORTED, "a short causal convolution has 2 to 8 taps, not %d", d->width);
+  if (d->packed && !starts) return fail(c, B200CONV_E_INVALID, "packed sequences without their offsets");
+  const bool any = d->sequences && d->length && d->C;
+  if (any && !x) return fail(c, B200CONV_E_INVALID, "causal convolution without input");
+  if (d->C && !w) return fail(c, B200CONV_E_INVALID, "causal convolution without filters");
+  return check_rows(c, "x", x, d->x, d->packed ? 1 : d->sequences, d->length, d->C);
+}
+static size_t causal_state_bytes(const b200conv_causal_desc* d) {
+  return row_elem_size(d->dtype) * static_cast<size_t>(d->sequences) * (d->width - 1) * d->C;
+}
+
+int b200conv_causal_conv(b200conv_ctx* c, const b200conv_causal_desc* d, const void* x, const void* w, const void* bias, const void* initial,
+                         const int32_t* starts, void* y, void* final) {
+  if (!c) return B200CONV_E_INVALID;
+  std::lock_guard<std::mutex> g(c->mu);
+  DeviceGuard dg(c->device);
+  int rc = check_causal(c, d, x, w, starts);
+  if (rc || (rc = check_rows(c, "y", y, d->y, d->packed ? 1 : d->sequences, d->length, d->C, true))) return rc;
+  if (!d->C || !d->sequences) return 0;
+  if (d->length && !y) return fail(c, B200CONV_E_INVALID, "causal convolution without output");
+  if (!d->length && !final) return 0;
+  Scratch tmp(c);
+  CausalArgs a = {};
+  a.d = *d;
+  a.x = x; a.w = w; a.bias = bias; a.initial = initial; a.starts = d->packed ? starts : nullptr; a.y = y; a.final = final;
+  if ((rc = detach_state(c, tmp, &a.initial, final, causal_state_bytes(d)))) return rc;
+  KLAUNCH(c, kKCausal, launch_causal_conv(a, c->stream));
+  return 0;
+}
+
+int b200conv_causal_conv_grad(b200conv_ctx* c, const b200conv_causal_desc* d, const void* dy, const void* x, const void* w, const void* bias,
+                              const void* initial, const int32_t* starts, void* dx, void* dw, void* dbias, void* dinitial) {
+  if (!c) return B200CONV_E_INVALID;
+  std::lock_guard<std::mutex> g(c->mu);
+  DeviceGuard dg(c->device);
+  int rc = check_causal(c, d, x, w, starts);
+  if (rc) return rc;
+  const long long n = d->packed ? 1 : d->sequences;
+  if ((rc = check_rows(c, "dy", dy, d->dy, n, d->length, d->C)) || (rc = check_rows(c, "dx", dx, d->dx, n, d->length, d->C, true))) return rc;
+  const size_t ps = d->param_f32 ? 4 : row_elem_size(d->dtype);
+  if (!d->C) return 0;
+  if (!d->sequences || !d->length) {                // sums over no tokens
+    if (dw) CU_OK(c, cudaMemsetAsync(dw, 0, ps * d->C * d->width, c->stream));
+    if (dbias) CU_OK(c, cudaMemsetAsync(dbias, 0, ps * d->C, c->stream));
+    if (dinitial && d->sequences) CU_OK(c, cudaMemsetAsync(dinitial, 0, causal_state_bytes(d), c->stream));
+    return 0;
+  }
+  if (!dy || !dx) return fail(c, B200CONV_E_INVALID, "causal convolution gradient without dy or dx");
+  Scratch tmp(c);
+  CausalArgs a = {};
+  a.d = *d;
+  a.dy = dy; a.x = x; a.w = w; a.bias = bias; a.initial = initial; a.starts = d->packed ? starts : nullptr;
+  a.dx = dx; a.dw = dw; a.dbias = dbias; a.dinitial = dinitial;
+  if ((dw || dbias) && (rc = tmp.get(sizeof(float) * (d->width + 1) * d->C * static_cast<size_t>(causal_grad_parts(a)),
+                                     reinterpret_cast<void**>(&a.partial))))
+    return rc;
+  int launches = 0;
+  KLAUNCH(c, kKCausal, launch_causal_grad(a, &launches, c->stream));
+  count_launches(c, launches - 1);
+  return 0;
+}
+
+int b200conv_causal_conv_step(b200conv_ctx* c, const b200conv_causal_desc* d, const void* x, const void* w, const void* bias, void* state, void* y) {
+  if (!c) return B200CONV_E_INVALID;
+  std::lock_guard<std::mutex> g(c->mu);
+  DeviceGuard dg(c->device);
+  if (d && (d->length != 1 || d->packed)) return fail(c, B200CONV_E_INVALID, "a step takes one token of every sequence");
+  int rc = check_causal(c, d, x, w, nullptr);
+  if (rc || (rc = check_rows(c, "y", y, d->y, d->sequences, 1, d->C, true))) return rc;
+  if (!d->C || !d->sequences) return 0;
+  if (!state || !y) return fail(c, B200CONV_E_INVALID, "causal convolution step without state or output");
+  CausalArgs a = {};
+  a.d = *d;
+  a.x = x; a.w = w; a.bias = bias; a.final = state; a.y = y;
+  KLAUNCH(c, kKCausal, launch_causal_step(a, c->stream));
   return 0;
 }
 

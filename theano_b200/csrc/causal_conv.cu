@@ -1,0 +1,131 @@
+// The short causal convolution: every channel with its own filter of 2 to 8 taps, bias and SiLU in the same pass.
+//
+//   pre[t][c] = bias[c] + sum over k of w[c][k] x[t - k][c],   y = pre or pre * sigmoid(pre)
+//
+// (a true convolution; without `flip` the taps are counted from the oldest token).  Tokens before a sequence's first are
+// the rows of its initial state, or zeros; the final state is the last taps - 1 rows of (initial state, x).
+// HBM bound: x is read once, y written once.  A thread takes V neighbouring channels (16 bytes) and walks along a run of
+// tokens with the last taps - 1 rows in registers; only those rows are read a second time, out of L2, by the next run.
+#include "causal_conv.cuh"
+#include "internal.h"
+
+namespace b200 {
+namespace {
+
+constexpr int kAhead = 4;                        // rows whose loads a thread has in flight
+
+template <typename T, int V, int K>
+__global__ void __launch_bounds__(256) causal_conv_kernel(CausalArgs a, CausalGrid g) {
+  pdl_enter();
+  if (blockIdx.x >= g.run_blocks) {              // the states behind the sequences, in blocks of their own
+    final_state<T, V, K>(a, blockIdx.x - g.run_blocks);
+    return;
+  }
+  const int c = ((blockIdx.x % g.channel_blocks << g.log_lanes) + (threadIdx.x & ((1 << g.log_lanes) - 1))) * V;
+  const long long run = (static_cast<long long>(blockIdx.x / g.channel_blocks) << (8 - g.log_lanes)) + (threadIdx.x >> g.log_lanes);
+  if (c >= a.d.C) return;
+  RunPlace p = place_run(a, g, run);
+  if (p.from >= p.to) return;
+  float w[K][V], bias[V];
+  load_filter<T, V, K>(a, c, w, bias);
+  const T* x = static_cast<const T*>(a.x) + p.seq * a.d.x.seq + c;
+  T* y = static_cast<T*>(a.y) + p.seq * a.d.y.seq + c;
+  Place at = place_token(a, p, p.from);
+  long long t = at.token;
+  if (t >= p.to) return;                         // rows of no sequence
+  float win[K - 1][V];
+  load_window<T, V, K>(a, x, at, t, c, win);
+  while (t < p.to) {
+    Pack<T, V> in[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (t + k < p.to) in[k].load(x + (t + k) * a.d.x.row);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      if (t + k >= p.to) break;
+      if (t + k >= at.end) {                     // packed sequences: the next one begins here, or rows of none
+        if (!next_sequence(a, t + k, &at)) return;
+        if (at.token == t + k) load_window<T, V, K>(a, x, at, t + k, c, win);
+      }
+      float now[V], out[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        now[i] = in[k].get(i);
+        float pre = bias[i] + w[0][i] * now[i];
+#pragma unroll
+        for (int j = 1; j < K; ++j) pre += w[j][i] * win[K - 1 - j][i];
+        out[i] = a.d.silu ? silu(pre) : pre;
+      }
+#pragma unroll
+      for (int j = 0; j + 2 < K; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) win[j][i] = win[j + 1][i];
+#pragma unroll
+      for (int i = 0; i < V; ++i) win[K - 2][i] = now[i];
+      store_row<T, V>(y + (t + k) * a.d.y.row, out);
+      if (c + V >= a.d.C)
+        for (int z = V; c + z < a.d.y.stored; ++z) y[(t + k) * a.d.y.row + z] = from_float<T>(0.f);
+    }
+    t += kAhead;
+  }
+}
+
+// One token of every sequence: reads the state and the token, leaves y and the state moved on by a row.
+template <typename T, int V, int K>
+__global__ void __launch_bounds__(128) causal_step_kernel(CausalArgs a, int vecs) {
+  pdl_enter();
+  const long long i = blockIdx.x * 128LL + threadIdx.x;
+  if (i >= a.d.sequences * vecs) return;
+  const long long seq = i / vecs;
+  const int c = static_cast<int>(i - seq * vecs) * V;
+  T* state = static_cast<T*>(a.final) + seq * (K - 1) * a.d.C + c;
+  Pack<T, V> old[K - 1], now;
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j) old[j].load(state + 1LL * j * a.d.C);
+  now.load(static_cast<const T*>(a.x) + seq * a.d.x.seq + c);
+  float w[K][V], bias[V], out[V];
+  load_filter<T, V, K>(a, c, w, bias);
+#pragma unroll
+  for (int q = 0; q < V; ++q) {
+    float pre = bias[q] + w[0][q] * now.get(q);
+#pragma unroll
+    for (int j = 1; j < K; ++j) pre += w[j][q] * old[K - 1 - j].get(q);
+    out[q] = a.d.silu ? silu(pre) : pre;
+  }
+#pragma unroll
+  for (int j = 0; j + 2 < K; ++j) old[j + 1].store(state + 1LL * j * a.d.C);
+  now.store(state + (K - 2LL) * a.d.C);
+  T* y = static_cast<T*>(a.y) + seq * a.d.y.seq + c;
+  store_row<T, V>(y, out);
+  if (c + V >= a.d.C)
+    for (int z = V; c + z < a.d.y.stored; ++z) y[z] = from_float<T>(0.f);
+}
+
+template <typename T, int V, int K>
+cudaError_t forward(const CausalArgs& a, cudaStream_t s) {
+  const CausalGrid g = causal_grid(a, V, 148 * 2048, kAhead, 32);
+  long long grid = g.run_blocks;
+  if (a.final) grid += (a.d.sequences * (K - 1) * (a.d.C / V) + 255) / 256;
+  if (grid >= INT32_MAX) return cudaErrorInvalidValue;
+  if (grid) launch_streaming(causal_conv_kernel<T, V, K>, static_cast<unsigned>(grid), 256, 0, s, a, g);
+  return cudaGetLastError();
+}
+template <typename T, int V, int K>
+cudaError_t step(const CausalArgs& a, cudaStream_t s) {
+  const int vecs = a.d.C / V;
+  const long long grid = (a.d.sequences * vecs + 127) / 128;
+  if (grid >= INT32_MAX) return cudaErrorInvalidValue;
+  launch_streaming(causal_step_kernel<T, V, K>, static_cast<unsigned>(grid), 128, 0, s, a, vecs);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_causal_conv(const CausalArgs& a, cudaStream_t s) {
+  return with_causal(a, wide_causal(a), [&](auto t, auto v, auto k) { return forward<decltype(t), decltype(v)::value, decltype(k)::value>(a, s); });
+}
+cudaError_t launch_causal_step(const CausalArgs& a, cudaStream_t s) {
+  return with_causal(a, wide_causal(a), [&](auto t, auto v, auto k) { return step<decltype(t), decltype(v)::value, decltype(k)::value>(a, s); });
+}
+
+}  // namespace b200

@@ -18,7 +18,7 @@ inline long long cdiv(long long a, long long b) { return (a + b - 1) / b; }
 inline size_t elem_size(int dtype) { return dtype == B200CONV_F16 ? 2 : 4; }
 // Channels-last tensors pad the channel count so that one pixel is a multiple of 16 bytes
 // (tensor-map strides must be).
-inline int pad_channels(int c, int dtype) { return round_up(c < 1 ? 1 : c, dtype == B200CONV_F16 ? 8 : 4); }
+inline int pad_channels(int c, int dtype) { return round_up(c < 1 ? 1 : c, dtype == B200CONV_F32 ? 4 : 8); }
 
 inline bool fits16(int v) { return v >= -32768 && v <= 32767; }
 

@@ -1,0 +1,477 @@
+"""Layers of sequence models on the GPU: layer norm, the short causal convolution and the selective state space scan.
+
+Beside the convolutions of ``theano_b200.shim`` and in the same two forms: numpy arrays in and out (what an op's
+``perform`` calls) and ``device_*`` calls on tensors that stay in HBM, which are asynchronous on their context's stream.
+Sequence tensors are ``(sequences, tokens, channels)`` with contiguous channels; sequences of several lengths may lie one
+behind the other in a ``(rows, channels)`` tensor (`Sequences`).  A channels-last ``shim.DeviceTensor`` counts as one with
+its pixels as tokens.  Data types: float32, float16 and bfloat16; sums and states are float32.
+
+The reference runs causal convolutions through its 2-D convolution (theano/tensor/nnet/abstract_conv.py, causal_conv1d) and
+recurrences through its scan op, one op call per token; nothing here computes on the CPU.
+"""
+import ctypes
+
+import numpy as np
+
+from . import shim
+from .shim import DeviceTensor, _P
+
+F32, F16, BF16 = shim.F32, shim.F16, 2
+# numpy has no bfloat16: its bits in a field of that name, so that no calculation takes them for integers
+BFLOAT16 = np.dtype([("bfloat16", np.uint16)])
+_CODES = {np.dtype(np.float32): F32, np.dtype(np.float16): F16, BFLOAT16: BF16}
+_DTYPES = {F32: np.dtype(np.float32), F16: np.dtype(np.float16), BF16: BFLOAT16}
+_INT32 = np.dtype(np.int32)
+_OTHER = -1                              # code of tensors that are no operands (offsets)
+
+
+def _dtype(dt):
+    return BFLOAT16 if isinstance(dt, str) and dt == "bfloat16" else np.dtype(dt)
+
+
+def to_bfloat16(a):
+    """float32 values as bfloat16 bits (`BFLOAT16`), rounded to nearest even."""
+    bits = np.ascontiguousarray(a, dtype=np.float32).view(np.uint32)
+    nan = (bits & 0x7fffffff) > 0x7f800000
+    out = ((bits + 0x7fff + ((bits >> 16) & 1)) >> 16).astype(np.uint16)
+    out[nan] = 0x7fc0
+    return out.view(BFLOAT16).reshape(np.shape(a))
+
+
+def from_bfloat16(a):
+    """The float32 values of bfloat16 bits."""
+    return (np.ascontiguousarray(a).view(np.uint16).astype(np.uint32) << 16).view(np.float32).reshape(np.shape(a))
+
+
+class DeviceArray(object):
+    """An array in HBM of up to four axes, the last one contiguous; ``strides`` are in elements.
+
+    ``a[:, 3:9]`` and the like are views (integers and slices of step 1), which keep the array alive.  Arrays that wrap a
+    pointer (``_ptr``) own nothing.  ``stored``: channels that a row holds in memory, those beyond the shape's last
+    extent being zeros that the operators write (pad channels of an image)."""
+
+    def __init__(self, ctx, shape, dtype, strides=None, _ptr=None, stored=0, _base=None):
+        self.ctx, self.shape, self.dtype = ctx, tuple(int(s) for s in shape), _dtype(dtype)
+        if not 1 <= len(self.shape) <= 4 or any(s < 0 for s in self.shape):
+            raise ValueError("a device array has one to four axes of extent 0 or more, not %s" % (self.shape,))
+        if strides is None:
+            strides, n = [], 1
+            for s in reversed(self.shape):
+                strides.insert(0, n)
+                n *= s
+        elif _ptr is None:
+            raise ValueError("strides belong to arrays that wrap memory")
+        self.strides = tuple(int(s) for s in strides)
+        if len(self.strides) != len(self.shape) or any(s < 0 for s in self.strides) or (self.shape[-1] > 1 and self.strides[-1] != 1):
+            raise ValueError("the last axis must be contiguous and no stride negative: shape %s, strides %s" % (self.shape, self.strides))
+        self.stored, self._base = int(stored), _base
+        self.code = _CODES.get(self.dtype, _OTHER)
+        self.sig = (self.shape, self.strides, self.code, self.stored)
+        self.owner = _ptr is None
+        self.ptr = ctx.malloc(self.size * self.dtype.itemsize) if self.owner else _ptr
+
+    @property
+    def size(self):
+        n = 1
+        for s in self.shape:
+            n *= s
+        return n
+
+    @property
+    def span(self):
+        """Elements from the first to behind the last one."""
+        return 1 + sum((n - 1) * s for n, s in zip(self.shape, self.strides)) if self.size else 0
+
+    def __getitem__(self, key):
+        key = key if isinstance(key, tuple) else (key,)
+        if len(key) > len(self.shape) or any(k is Ellipsis or k is None for k in key):
+            raise IndexError("too many indices, or neither integers nor slices")
+        shape, strides, at = [], [], 0
+        for axis, n in enumerate(self.shape):
+            k = key[axis] if axis < len(key) else slice(None)
+            if isinstance(k, slice):
+                a, b, step = k.indices(n)
+                if step != 1:
+                    raise IndexError("slices of a device array have step 1")
+                shape.append(max(0, b - a))
+                strides.append(self.strides[axis])
+                at += a * self.strides[axis]
+            else:
+                k = k.__index__()
+                if not -n <= k < n or axis == len(self.shape) - 1:
+                    raise IndexError("index %d of axis %d (extent %d; the last axis takes slices)" % (k, axis, n))
+                at += (k % n) * self.strides[axis]
+        whole = shape[-1] == self.shape[-1]
+        return DeviceArray(self.ctx, shape, self.dtype, strides, (self.ptr or 0) + at * self.dtype.itemsize, self.stored if whole else 0, self)
+
+    @classmethod
+    def rows_of(cls, image):
+        """The (N, H * W, C) rows of a channels-last `shim.DeviceTensor`."""
+        if image.layout != "nhwc":
+            raise ValueError("sequence operators take channels-last tensors")
+        n, c, h, w = image.shape
+        cp = image.stored_channels
+        return cls(image.ctx, (n, h * w, c), image.dtype, (h * w * cp, cp, 1), image.ptr, cp, image)
+
+    @classmethod
+    def from_host(cls, ctx, arr, dtype=None):
+        """Upload a numpy array, as `dtype` (default: its own; 'bfloat16' rounds float32 values)."""
+        dtype = _dtype(arr.dtype if dtype is None else dtype)
+        arr = np.ascontiguousarray(arr)
+        if arr.dtype != dtype:
+            arr = to_bfloat16(arr) if dtype == BFLOAT16 else arr.astype(dtype)
+        t = cls(ctx, arr.shape or (1,), dtype)
+        ctx.h2d(t.ptr, arr)
+        ctx.sync()
+        return t
+
+    def to_host(self):
+        """A numpy array of the values (bfloat16: as float32)."""
+        flat = np.empty(self.span, self.dtype)
+        self.ctx.d2h(flat, self.ptr)
+        self.ctx.sync()
+        es = self.dtype.itemsize
+        if not self.size:
+            a = np.empty(self.shape, self.dtype)
+        else:
+            a = np.array(np.lib.stride_tricks.as_strided(flat, self.shape, [s * es for s in self.strides]))
+        return from_bfloat16(a) if self.dtype == BFLOAT16 else a
+
+    def free(self):
+        if self.ptr and self.owner:
+            self.ctx.free(self.ptr)
+        self.ptr = None
+
+    def __del__(self):
+        try:
+            if self.owner and self.ctx.h:
+                self.free()
+        except Exception:
+            pass
+
+
+class Sequences(object):
+    """The lengths of sequences that lie one behind the other in the rows of a (rows, channels) tensor; rows behind the
+    last sequence belong to none: they are neither read nor written.  Made once per batch and kept by the program."""
+
+    def __init__(self, ctx, lengths):
+        lengths = np.asarray(lengths)
+        if lengths.ndim != 1 or lengths.size == 0 or lengths.dtype.kind not in "iu":
+            raise ValueError("lengths must be a vector of integers with one entry or more")
+        if lengths.min() < 0 or int(lengths.astype(np.int64).sum()) > np.iinfo(np.int32).max:
+            raise ValueError("lengths must not be negative nor add up to over 2^31 - 1")
+        self.ctx, self.count = ctx, int(lengths.size)
+        self.lengths = tuple(int(n) for n in lengths)
+        self.total, self.longest = int(lengths.astype(np.int64).sum()), int(lengths.max())
+        self.starts = DeviceArray.from_host(ctx, np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32))
+        self.sig = (self.count, self.total, self.longest)
+
+
+# ======================================================================================
+# plans: descriptors of calls that have been checked
+# ======================================================================================
+class Rows(ctypes.Structure):
+    """``b200conv_rows`` of include/b200conv.h."""
+    _fields_ = [("row", ctypes.c_int64), ("seq", ctypes.c_int64), ("stored", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class NormDesc(ctypes.Structure):
+    """``b200conv_norm_desc``."""
+    _fields_ = [("sequences", ctypes.c_int64), ("length", ctypes.c_int64), ("C", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("param_f32", ctypes.c_int32), ("eps", ctypes.c_float)] + [
+                    (n, Rows) for n in ("x", "residual", "y", "total", "dy", "dtotal", "dx")]
+
+
+_plans = {}                              # signature of a call -> its checked descriptor; emptied when it holds _LIMIT
+_LIMIT = 4096
+
+
+def _plan(key, make, *args):
+    plan = _plans.get(key)
+    if plan is None:
+        plan = make(*args)
+        if len(_plans) >= _LIMIT:
+            _plans.clear()
+        _plans[key] = plan
+    return plan
+
+
+def _array(t):
+    """A tensor argument as a DeviceArray: channels-last images as their rows, other DeviceTensors as a vector."""
+    if t is None or type(t) is DeviceArray:
+        return t
+    if isinstance(t, DeviceTensor):
+        if t.layout == "nhwc":
+            return DeviceArray.rows_of(t)
+        n = t.shape[0] * t.shape[1] * t.shape[2] * t.shape[3]
+        return DeviceArray(t.ctx, (n,), t.dtype, (1,), t.ptr, 0, t)
+    if isinstance(t, DeviceArray):
+        return t
+    raise TypeError("expected a DeviceArray or a channels-last DeviceTensor, not %s" % type(t).__name__)
+
+
+def _sig(t):
+    return None if t is None else t.sig
+
+
+def _ptr(t):
+    return None if t is None else t.ptr
+
+
+def _one_context(ctx, *tensors):
+    for t in tensors:
+        if t is not None and t.ctx is not ctx:
+            raise ValueError("tensors of one call must belong to one context (another context's stream is not waited for)")
+
+
+def _like(t, original):
+    """A new tensor for a result of `t`'s shape: an image where the argument was one."""
+    if isinstance(original, DeviceTensor):
+        return DeviceTensor(t.ctx, original.shape, t.dtype, "nhwc")
+    return DeviceArray(t.ctx, t.shape, t.dtype)
+
+
+def _same(what, t, shape, code):
+    if t is None:
+        return
+    if t.shape != tuple(shape):
+        raise ValueError("%s must have shape %s, not %s" % (what, tuple(shape), t.shape))
+    if t.code != code:
+        raise TypeError("%s must be %s, not %s" % (what, _DTYPES[code], t.dtype))
+
+
+def _operand_code(t):
+    if t.code == _OTHER:
+        raise TypeError("sequence operators handle float32, float16 and bfloat16, not %s" % t.dtype)
+    return t.code
+
+
+def _params(what, code, *tensors):
+    """Whether the parameters are float32 beside tensors of another type; all of them share one."""
+    codes = {t.code for t in tensors if t is not None}
+    if len(codes) > 1 or not codes <= {code, F32}:
+        raise TypeError("%s must share one data type: the tensors' or float32" % what)
+    return int(code != F32 and codes == {F32})
+
+
+def _rows(t):
+    if t is None:
+        return Rows()
+    seq, row = (t.strides[0], t.strides[1]) if len(t.shape) == 3 else (0, t.strides[0])
+    return Rows(row, seq, t.stored, 0)
+
+
+# ======================================================================================
+# layer norm
+# ======================================================================================
+def _norm_shape(x):
+    if len(x.shape) not in (2, 3):
+        raise ValueError("layer norm takes (rows, channels) or (sequences, tokens, channels), not %s" % (x.shape,))
+    return (x.shape[:2] if len(x.shape) == 3 else (1, x.shape[0])) + (x.shape[-1],)
+
+
+def _plan_norm(eps, x, gamma, beta, stats, **tensors):
+    code = _operand_code(x)
+    S, T, C = _norm_shape(x)
+    if C == 0:
+        raise ValueError("layer norm over no channels")
+    if not eps >= 0:
+        raise ValueError("eps must not be negative")
+    for name, t in tensors.items():
+        _same(name, t, x.shape, code)
+    for name, t in (("gamma", gamma), ("beta", beta)):
+        if t is not None and t.shape != (C,):
+            raise ValueError("%s must have one value per channel (%d), not shape %s" % (name, C, t.shape))
+    _same("stats", stats, x.shape[:-1] + (2,), F32)
+    if stats is not None and stats.strides != DeviceArray(x.ctx, stats.shape, np.float32, _ptr=0).strides:
+        raise ValueError("stats must be contiguous")
+    d = NormDesc(S, T, C, code, _params("gamma and beta", code, gamma, beta), eps)
+    d.x = _rows(x)
+    for name, t in tensors.items():
+        setattr(d, name, _rows(t))
+    return ctypes.byref(d)
+
+
+def device_layer_norm(x, gamma=None, beta=None, eps=1e-5, residual=None, total=None, stats=None, out=None):
+    """Layer norm over the channels of every row of x (+ residual): ``(t - mean) * rstd * gamma + beta``.
+
+    `gamma`, `beta`: vectors of the tensors' type or float32.  `residual`: added to x first; `total` receives the sum,
+    rounded to the tensors' type, which is what is normalised (it may be x or residual themselves).  `stats`: float32 of
+    x's shape with (mean, rstd) in place of the channels, for the gradient.  Returns `out` (which may be x)."""
+    given, x = x, _array(x)
+    ctx = x.ctx
+    gamma, beta, residual, total, stats = _array(gamma), _array(beta), _array(residual), _array(total), _array(stats)
+    if out is None:
+        out = _like(x, given)
+    y = _array(out)
+    _one_context(ctx, gamma, beta, residual, total, stats, y)
+    d = _plan(("norm", eps, x.sig, _sig(gamma), _sig(beta), _sig(stats), _sig(residual), _sig(total), y.sig), lambda: _plan_norm(
+        eps, x, gamma, beta, stats, residual=residual, total=total, y=y))
+    rc = ctx.lib.b200conv_layer_norm(ctx.h, d, x.ptr, _ptr(residual), _ptr(gamma), _ptr(beta), y.ptr, _ptr(total), _ptr(stats))
+    if rc:
+        ctx.check(rc)
+    return out
+
+
+def device_layer_norm_grad(dy, x, gamma, stats, dtotal=None, out=None, dgamma=None, dbeta=None):
+    """Gradients (dx, dgamma, dbeta) of `device_layer_norm`; x is what was normalised (`total` where there was a
+    residual) and `stats` what the forward call left.  `dtotal`, the gradient that reaches the sum on other ways, is added to
+    dx, which may be dy or dtotal.  dgamma and dbeta have gamma's type (float32 without one); False leaves one out."""
+    given, dy = dy, _array(dy)
+    ctx = dy.ctx
+    x, gamma, stats, dtotal = _array(x), _array(gamma), _array(stats), _array(dtotal)
+    if out is None:
+        out = _like(dy, given)
+    ptype = gamma.dtype if gamma is not None else np.float32
+    grads = [None if g is False else g if g is not None else DeviceArray(ctx, (dy.shape[-1],), ptype) for g in (dgamma, dbeta)]
+    dg, db = (_array(g) for g in grads)
+    dx = _array(out)
+    _one_context(ctx, x, gamma, stats, dtotal, dx, dg, db)
+    if stats is None:
+        raise ValueError("the gradient needs the statistics of the forward call")
+
+    def make():
+        _params("gamma and its gradients", dy.code, gamma, dg, db)
+        for name, t in (("dgamma", dg), ("dbeta", db)):
+            if t is not None and t.shape != (dy.shape[-1],):
+                raise ValueError("%s must have one value per channel (%d), not shape %s" % (name, dy.shape[-1], t.shape))
+        d = _plan_norm(0.0, x, gamma, None, stats, dy=dy, dtotal=dtotal, dx=dx)
+        d._obj.param_f32 = _params("gamma and its gradients", dy.code, gamma, dg, db)
+        return d
+    d = _plan(("norm grad", dy.sig, x.sig, _sig(gamma), stats.sig, _sig(dtotal), dx.sig, _sig(dg), _sig(db)), make)
+    rc = ctx.lib.b200conv_layer_norm_grad(ctx.h, d, dy.ptr, x.ptr, _ptr(gamma), stats.ptr, _ptr(dtotal), dx.ptr, _ptr(dg), _ptr(db))
+    if rc:
+        ctx.check(rc)
+    return out, grads[0], grads[1]
+
+
+# ======================================================================================
+# the short causal convolution
+# ======================================================================================
+class CausalDesc(ctypes.Structure):
+    """``b200conv_causal_desc``."""
+    _fields_ = [("sequences", ctypes.c_int64), ("length", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in (
+        "C", "width", "dtype", "param_f32", "flip", "silu", "packed", "reserved")] + [(n, Rows) for n in ("x", "y", "dy", "dx")]
+
+
+def _contiguous(what, t):
+    if t is not None:
+        n = 1
+        for size, stride in zip(reversed(t.shape), reversed(t.strides)):
+            if size > 1 and stride != n:
+                raise ValueError("%s must be contiguous" % what)
+            n *= size
+
+
+def _batch(x, sequences, what):
+    """(sequences, tokens of each or rows of the tensor, channels) of a call's main tensor."""
+    if sequences is None:
+        if len(x.shape) != 3:
+            raise ValueError("%s takes (sequences, tokens, channels), not %s" % (what, x.shape))
+        return x.shape[0], x.shape[1], x.shape[2]
+    if len(x.shape) != 2:
+        raise ValueError("%s takes packed sequences as (rows, channels), not %s" % (what, x.shape))
+    if sequences.total > x.shape[0]:
+        raise ValueError("the sequences have %d tokens, the tensor has %d rows" % (sequences.total, x.shape[0]))
+    return sequences.count, x.shape[0], x.shape[1]
+
+
+def _plan_causal(x, w, bias, silu, flip, packed, S, T, C, states, tensors, grads):
+    code = _operand_code(x)
+    if len(w.shape) != 2 or w.shape[0] != C:
+        raise ValueError("the filters must have shape (%d, taps), not %s" % (C, w.shape))
+    width = w.shape[1]
+    if not 2 <= width <= 8:
+        raise ValueError("a short causal convolution has 2 to 8 taps, not %d" % width)
+    _contiguous("the filters", w)
+    if bias is not None and bias.shape != (C,):
+        raise ValueError("bias must have one value per channel (%d), not shape %s" % (C, bias.shape))
+    for name, t, like in grads:
+        if t is not None and t.shape != like:
+            raise ValueError("%s must have shape %s, not %s" % (name, like, t.shape))
+        _contiguous(name, t)
+    for name, t in states:
+        _same(name, t, (S, width - 1, C), code)
+        _contiguous(name, t)
+    for name, t in tensors:
+        _same(name, t, x.shape, code)
+    d = CausalDesc(S, T, C, width, code, _params("filters, bias and their gradients", code, w, bias, *[t for _, t, _ in grads]), int(bool(flip)),
+                   int(bool(silu)), int(packed), 0)
+    d.x = _rows(x)
+    for name, t in tensors:
+        if t is not None:
+            setattr(d, name, _rows(t))
+    return ctypes.byref(d)
+
+
+def device_causal_conv1d(x, w, bias=None, silu=False, filter_flip=True, initial=None, final=None, sequences=None, out=None):
+    """Every channel's own short filter over the tokens up to each one: ``y[t] = sum_k w[:, k] x[t - k]`` (without
+    `filter_flip` the last weight meets token t), + `bias`, then v * sigmoid(v) with `silu`.
+
+    `w`: (channels, taps), 2 to 8 taps; `initial`: (sequences, taps - 1, channels), the tokens before the first, oldest
+    first (default: zeros); `final` receives the same behind the last token and may be `initial`.  With `sequences`
+    x is (rows, channels).  Returns `out`."""
+    given, x, w, bias = x, _array(x), _array(w), _array(bias)
+    ctx = x.ctx
+    initial, final = _array(initial), _array(final)
+    if out is None:
+        out = _like(x, given)
+    y = _array(out)
+    _one_context(ctx, w, bias, initial, final, y, sequences)
+    d = _plan(("causal", silu, filter_flip, x.sig, w.sig, _sig(bias), _sig(initial), _sig(final), y.sig, _sig(sequences)), lambda: _plan_causal(
+        x, w, bias, silu, filter_flip, sequences is not None, *_batch(x, sequences, "a causal convolution"),
+        (("initial", initial), ("final", final)), (("y", y),), ()))
+    rc = ctx.lib.b200conv_causal_conv(ctx.h, d, x.ptr, w.ptr, _ptr(bias), _ptr(initial), sequences and sequences.starts.ptr, y.ptr, _ptr(final))
+    if rc:
+        ctx.check(rc)
+    return out
+
+
+def device_causal_conv1d_grad(dy, x, w, bias=None, silu=False, filter_flip=True, initial=None, sequences=None, out=None, dw=None, dbias=None,
+                              dinitial=None):
+    """Gradients (dx, dw, dbias, dinitial) of `device_causal_conv1d`.  dw and dbias have the types of w and bias (False
+    leaves one out, dbias exists with a bias only), dinitial is computed where it is given."""
+    given, dy, x, w, bias = dy, _array(dy), _array(x), _array(w), _array(bias)
+    ctx = x.ctx
+    initial, dinitial = _array(initial), _array(dinitial)
+    if out is None:
+        out = _like(dy, given)
+    dx = _array(out)
+    dw = None if dw is False else dw if dw is not None else DeviceArray(ctx, w.shape, w.dtype)
+    dbias = None if dbias is False or bias is None else dbias if dbias is not None else DeviceArray(ctx, bias.shape, bias.dtype)
+    gw, gb = _array(dw), _array(dbias)
+    _one_context(ctx, dy, w, bias, initial, dx, gw, gb, dinitial, sequences)
+    d = _plan(("causal grad", silu, filter_flip, dy.sig, x.sig, w.sig, _sig(bias), _sig(initial), dx.sig, _sig(gw), _sig(gb), _sig(dinitial),
+               _sig(sequences)), lambda: _plan_causal(
+        x, w, bias, silu, filter_flip, sequences is not None, *_batch(x, sequences, "a causal convolution"),
+        (("initial", initial), ("dinitial", dinitial)), (("dy", dy), ("dx", dx)),
+        (("dw", gw, w.shape), ("dbias", gb, (w.shape[0],)))))
+    rc = ctx.lib.b200conv_causal_conv_grad(ctx.h, d, dy.ptr, x.ptr, w.ptr, _ptr(bias), _ptr(initial), sequences and sequences.starts.ptr, dx.ptr,
+                                           _ptr(gw), _ptr(gb), _ptr(dinitial))
+    if rc:
+        ctx.check(rc)
+    return out, dw, dbias, dinitial
+
+
+def device_causal_conv1d_step(x, state, w, bias=None, silu=False, filter_flip=True, out=None):
+    """One token of every sequence, x (sequences, channels): the token `device_causal_conv1d` would give behind `state`,
+    (sequences, taps - 1, channels), which moves on in place.  `out` may be x."""
+    x, w, bias, state = _array(x), _array(w), _array(bias), _array(state)
+    ctx = x.ctx
+    if out is None:
+        out = DeviceArray(ctx, x.shape, x.dtype)
+    y = _array(out)
+    _one_context(ctx, w, bias, state, y)
+
+    def make():
+        if len(x.shape) != 2:
+            raise ValueError("a step takes (sequences, channels), not %s" % (x.shape,))
+        d = _plan_causal(x, w, bias, silu, filter_flip, False, x.shape[0], 1, x.shape[1], (("state", state),), (("y", y),), ())
+        for name, t in (("x", x), ("y", y)):
+            setattr(d._obj, name, Rows(x.shape[1], t.strides[0], t.stored, 0))
+        return d
+    d = _plan(("causal step", silu, filter_flip, x.sig, w.sig, _sig(bias), state.sig, y.sig), make)
+    rc = ctx.lib.b200conv_causal_conv_step(ctx.h, d, x.ptr, w.ptr, _ptr(bias), state.ptr, y.ptr)
+    if rc:
+        ctx.check(rc)
+    return out

@@ -60,6 +60,11 @@ SIGNATURES = {
     "b200conv_maxpool2x2_grad": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I]),
     "b200conv_elementwise": (_I, [_P, _I, _P, _P, _P, ctypes.c_longlong, _I, _I, ctypes.c_float, _I]),
     "b200conv_channel_sum": (_I, [_P, _P, _P, ctypes.c_longlong, _I, _I]),
+    "b200conv_layer_norm": (_I, [_P] * 9),
+    "b200conv_layer_norm_grad": (_I, [_P] * 10),
+    "b200conv_causal_conv": (_I, [_P] * 9),
+    "b200conv_causal_conv_grad": (_I, [_P] * 12),
+    "b200conv_causal_conv_step": (_I, [_P] * 7),
     "b200conv_padded_channels": (_I, [_I, _I]),
     "b200conv_malloc": (_I, [_P, _SZ, ctypes.POINTER(_P)]),
     "b200conv_free": (_I, [_P, _P]),
