@@ -282,6 +282,37 @@ int b200conv_causal_conv_grad(b200conv_ctx* ctx, const b200conv_causal_desc* d, 
 int b200conv_causal_conv_step(b200conv_ctx* ctx, const b200conv_causal_desc* d, const void* x, const void* w,
                               const void* bias, void* state, void* y);
 
+/* Selective state space scan: N states per channel, which decay and are driven by step sizes that depend on the token.
+ *   delta = dt + dt_bias, with softplus log(1 + exp(.)) of it
+ *   h[t][c][n] = exp(delta[t][c] * A[c][n]) * h[t - 1][c][n] + delta[t][c] * x[t][c] * B[t][g][n]
+ *   y[t][c] = (sum over n of C[t][g][n] * h[t][c][n] + D[c] * x[t][c]) * (z ? z * sigmoid(z) : 1)
+ * for channels c of group g = c / (C / groups).  x, dt, z, y have C channels, B and C rows of groups * N elements; A [C][N], D and
+ * dt_bias [C] are float32; D, z and dt_bias may be NULL.  A is at most 0 and delta at least 0 in such layers; results follow the formulas
+ * elsewhere too, as far as float32 reaches.  1 <= N <= 128.  initial and final: float32 states [sequences][C][N] before the
+ * first (NULL: zeros) and behind the last token; they may be one array.  Packed sequences as above; `longest` is an upper bound of their
+ * lengths that only guides the cut of the work (0: not known).
+ * The gradient takes the forward call's inputs, dy and, where given, dfinal (like final), and writes dx, ddt, dA, dB, dC, dz (with z), and
+ * where given dD, ddt_bias and dinitial (like initial); rows of no sequence are left as they were.  Its workspace is one float32 state per
+ * eight tokens and channel and, for every 4 * floor(128 / L) channels of a group (L: lanes of a channel, 4 up to N = 16, 8, 16, 32 up to
+ * N = 128), one pair of float32 B and C rows per token.
+ * The step takes one token of every sequence (length 1) and moves `state`, like initial, on in place; y may be x, dt or z. */
+typedef struct b200conv_scan_desc {
+  int64_t sequences, length;
+  int32_t C, N, groups, dtype, softplus, packed, longest, reserved;
+  b200conv_rows x, dt, z, B, Cm, y, dy, dx, ddt, dz, dB, dCm;
+} b200conv_scan_desc;
+int b200conv_selective_scan(b200conv_ctx* ctx, const b200conv_scan_desc* d, const void* x, const void* dt, const float* A,
+                            const void* B, const void* C, const float* D, const void* z, const float* dt_bias,
+                            const float* initial, const int32_t* starts, void* y, float* final);
+int b200conv_selective_scan_grad(b200conv_ctx* ctx, const b200conv_scan_desc* d, const void* dy, const void* x, const void* dt,
+                                 const float* A, const void* B, const void* C, const float* D, const void* z,
+                                 const float* dt_bias, const float* initial, const float* dfinal, const int32_t* starts,
+                                 void* dx, void* ddt, float* dA, void* dB, void* dC, float* dD, void* dz, float* ddt_bias,
+                                 float* dinitial);
+int b200conv_selective_scan_step(b200conv_ctx* ctx, const b200conv_scan_desc* d, const void* x, const void* dt, const float* A,
+                                 const void* B, const void* C, const float* D, const void* z, const float* dt_bias,
+                                 float* state, void* y);
+
 /* ---- device-resident tensors -------------------------------------------------------- */
 /* Channel count of the channels-last device layout (rounded up to 16 bytes). */
 int b200conv_padded_channels(int C, int dtype);

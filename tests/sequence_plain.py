@@ -74,48 +74,52 @@ def causal_conv_grad(dys, xs, w, bias, silu, flip, initials=None):
     return dxs, dw if flip else dw[:, ::-1], db, np.stack(dinits)
 
 
-def selective_scan(xs, dts, A, Bs, Cs, D=None, zs=None, dt_bias=None, softplus=False, initials=None, dys=None, dfinals=None):
-    """Sequences: x, dt, z [T][C], B, C [T][G][N].  -> dict(y=[...], final) and, with dys, the gradients."""
+def selective_scan(xs, dts, A, Bs, Cs, D=None, zs=None, dt_bias=None, softplus=False, initials=None, dys=None, dfinals=None, magnitudes=False):
+    """Sequences: x, dt, z [T][C], B, C [T][G][N].  -> dict(y=[...], final) and, with dys, the gradients.  `magnitudes`: every sum with
+    the magnitudes of its terms (the decays as they are), which bounds what relative errors of the factors can do."""
+    mag = np.abs if magnitudes else lambda v: v
     A = A.astype(np.float64)
     channels, N = A.shape
     out = dict(y=[], final=[])
     grads = {k: [] for k in ("x", "dt", "z", "B", "C", "initial")}
     grads.update(A=np.zeros(A.shape), D=np.zeros(channels), dt_bias=np.zeros(channels))
-    D64 = np.zeros(channels) if D is None else D.astype(np.float64)
+    D64 = np.zeros(channels) if D is None else mag(D.astype(np.float64))
     for i in range(len(xs)):
         x, dt, B, C = (np.asarray(v[i], np.float64) for v in (xs, dts, Bs, Cs))
         T, G = len(x), B.shape[1]
         share = np.arange(channels) // (channels // G)
         raw = dt + (0 if dt_bias is None else dt_bias.astype(np.float64))
         delta = np.logaddexp(0, raw) if softplus else raw
-        h = np.zeros((channels, N)) if initials is None else initials[i].astype(np.float64)
+        decay = np.exp(delta[..., None] * A)
+        x, B, C, delta = mag(x), mag(B), mag(C), mag(delta)
+        h = np.zeros((channels, N)) if initials is None else mag(initials[i].astype(np.float64))
         hs, first = [], h
         y0 = np.zeros(x.shape)
         for t in range(T):
-            h = np.exp(delta[t, :, None] * A) * h + (delta[t] * x[t])[:, None] * B[t, share]
+            h = decay[t] * h + (delta[t] * x[t])[:, None] * B[t, share]
             hs.append(h)
             y0[t] = (h * C[t, share]).sum(-1) + D64 * x[t]
         z = None if zs is None else np.asarray(zs[i], np.float64)
-        out["y"].append(y0 if z is None else y0 * z * sigmoid(z))
+        out["y"].append(y0 if z is None else y0 * mag(z * sigmoid(z)))
         out["final"].append(h)
         if dys is None:
             continue
-        dy = np.asarray(dys[i], np.float64)
+        dy = mag(np.asarray(dys[i], np.float64))
         if z is not None:
             s = sigmoid(z)
-            grads["z"].append(dy * y0 * s * (1 + z * (1 - s)))
-            dy = dy * z * s
-        lam = np.zeros((channels, N)) if dfinals is None else dfinals[i].astype(np.float64).copy()
+            grads["z"].append(dy * y0 * (s + np.abs(z) * s * (1 - s) if magnitudes else s * (1 + z * (1 - s))))
+            dy = dy * mag(z * s)
+        lam = np.zeros((channels, N)) if dfinals is None else mag(dfinals[i].astype(np.float64))
         dx, ddelta, dB, dC = D64 * dy, np.zeros(x.shape), np.zeros(B.shape), np.zeros(C.shape)
         for t in range(T - 1, -1, -1):
             lam = lam + dy[t][:, None] * C[t, share]
             dC[t] = (dy[t][:, None] * hs[t]).reshape(G, -1, N).sum(1)
             dB[t] = (lam * (delta[t] * x[t])[:, None]).reshape(G, -1, N).sum(1)
             lb = (lam * B[t, share]).sum(-1)
-            lam = lam * np.exp(delta[t, :, None] * A)
+            lam = lam * decay[t]
             through = lam * (hs[t - 1] if t else first)
             grads["A"] += through * delta[t, :, None]
-            ddelta[t] = (through * A).sum(-1) + x[t] * lb
+            ddelta[t] = (through * mag(A)).sum(-1) + x[t] * lb
             dx[t] += delta[t] * lb
         draw = ddelta * sigmoid(raw) if softplus else ddelta
         for k, v in (("x", dx), ("dt", draw), ("B", dB), ("C", dC), ("initial", lam)):

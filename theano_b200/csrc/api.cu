@@ -190,9 +190,9 @@ int fail(b200conv_ctx* c, int code, const char* fmt, ...) {
   } while (0)
 
 // Kernel families, for the launch counter and the optional per-kernel timing.
-enum { kKConvUmma = 0, kKWgradUmma, kKWgradReduce, kKTranspose, kKPack, kKDirect, kKPool, kKConvReduce, kKNorm, kKCausal, kKCount };
+enum { kKConvUmma = 0, kKWgradUmma, kKWgradReduce, kKTranspose, kKPack, kKDirect, kKPool, kKConvReduce, kKNorm, kKCausal, kKScan, kKCount };
 const char* const kKernelNames[kKCount] = {"conv_umma", "wgrad_umma", "wgrad_reduce", "transpose",
-                                           "pack", "direct", "pool", "conv_reduce", "layer_norm", "causal_conv"};
+                                           "pack", "direct", "pool", "conv_reduce", "layer_norm", "causal_conv", "selective_scan"};
 
 cudaEvent_t prof_event(b200conv_ctx* c) {
   cudaEvent_t e = nullptr;
@@ -3547,6 +3547,141 @@ int b200conv_causal_conv_step(b200conv_ctx* c, const b200conv_causal_desc* d, co
   a.d = *d;
   a.x = x; a.w = w; a.bias = bias; a.final = state; a.y = y;
   KLAUNCH(c, kKCausal, launch_causal_step(a, c->stream));
+  return 0;
+}
+
+static int check_scan(b200conv_ctx* c, const b200conv_scan_desc* d, const void* x, const void* dt, const float* A, const void* B, const void* C, const void* z,
+                      const int32_t* starts) {
+  if (!d) return fail(c, B200CONV_E_INVALID, "null descriptor");
+  const long long n = d->packed ? 1 : d->sequences;
+  int rc = check_sizes(c, n, d->length, d->C, d->dtype);
+  if (rc) return rc;
+  if (d->sequences < 0 || d->sequences > INT32_MAX / 8) return fail(c, B200CONV_E_INVALID, "%lld sequences", (long long)d->sequences);
+  if (d->N < 1 || d->N > 128) return fail(c, B200CONV_E_UNSUPPORTED, "a selective scan has 1 to 128 states per channel, not %d", d->N);
+  if (d->groups < 1 || d->C % d->groups) return fail(c, B200CONV_E_INVALID, "%d channels in %d groups", d->C, d->groups);
+  if (d->packed && !starts) return fail(c, B200CONV_E_INVALID, "packed sequences without their offsets");
+  if (!d->C || !d->sequences) return 0;
+  if (!A) return fail(c, B200CONV_E_INVALID, "selective scan without A");
+  if (d->length && (!x || !dt || !B || !C)) return fail(c, B200CONV_E_INVALID, "selective scan without x, dt, B or C");
+  if (d->y.stored > d->C || d->dx.stored > d->C || d->ddt.stored > d->C || d->dz.stored > d->C)
+    return fail(c, B200CONV_E_UNSUPPORTED, "a selective scan writes no pad channels");
+  const int gn = d->groups * d->N;
+  if ((rc = check_rows(c, "x", x, d->x, n, d->length, d->C)) || (rc = check_rows(c, "dt", dt, d->dt, n, d->length, d->C)) ||
+      (rc = check_rows(c, "z", z, d->z, n, d->length, d->C)) || (rc = check_rows(c, "B", B, d->B, n, d->length, gn)))
+    return rc;
+  return check_rows(c, "C", C, d->Cm, n, d->length, gn);
+}
+
+int b200conv_selective_scan(b200conv_ctx* c, const b200conv_scan_desc* d, const void* x, const void* dt, const float* A, const void* B, const void* C,
+                            const float* D, const void* z, const float* dt_bias, const float* initial, const int32_t* starts, void* y, float* final) {
+  if (!c) return B200CONV_E_INVALID;
+  std::lock_guard<std::mutex> g(c->mu);
+  DeviceGuard dg(c->device);
+  int rc = check_scan(c, d, x, dt, A, B, C, z, starts);
+  if (rc || (rc = check_rows(c, "y", y, d->y, d->packed ? 1 : d->sequences, d->length, d->C, true))) return rc;
+  if (!d->C || !d->sequences) return 0;
+  if (d->length && !y) return fail(c, B200CONV_E_INVALID, "selective scan without output");
+  const size_t state_bytes = sizeof(float) * static_cast<size_t>(d->sequences) * d->C * d->N;
+  if (!d->length) {                                 // the states pass through
+    if (!final || final == initial) return 0;
+    if (initial) CU_OK(c, cudaMemcpyAsync(final, initial, state_bytes, cudaMemcpyDeviceToDevice, c->stream));
+    else CU_OK(c, cudaMemsetAsync(final, 0, state_bytes, c->stream));
+    return 0;
+  }
+  Scratch tmp(c);
+  ScanArgs a = {};
+  a.d = *d;
+  a.x = x; a.dt = dt; a.A = A; a.B = B; a.C = C; a.D = D; a.z = z; a.dt_bias = dt_bias; a.initial = initial;
+  a.starts = d->packed ? starts : nullptr; a.y = y; a.final = final;
+  plan_scan_pieces(&a);
+  if (a.piece < d->length) {
+    const size_t n = static_cast<size_t>(a.pieces) * d->C, slots = scan_state_slots(d->N);
+    if ((rc = tmp.get(sizeof(float) * n * slots, reinterpret_cast<void**>(&a.piece_state))) ||
+        (rc = tmp.get(sizeof(float) * n, reinterpret_cast<void**>(&a.piece_sum))))
+      return rc;
+    const void* init = initial;
+    if ((rc = detach_state(c, tmp, &init, final, state_bytes))) return rc;
+    a.initial = static_cast<const float*>(init);
+  } else if (initial != final) {
+    const void* init = initial;
+    if ((rc = detach_state(c, tmp, &init, final, state_bytes))) return rc;
+    a.initial = static_cast<const float*>(init);
+  }
+  int launches = 0;
+  KLAUNCH(c, kKScan, launch_selective_scan(a, &launches, c->stream));
+  count_launches(c, launches - 1);
+  return 0;
+}
+
+int b200conv_selective_scan_grad(b200conv_ctx* c, const b200conv_scan_desc* d, const void* dy, const void* x, const void* dt, const float* A,
+                                 const void* B, const void* C, const float* D, const void* z, const float* dt_bias, const float* initial,
+                                 const float* dfinal, const int32_t* starts, void* dx, void* ddt, float* dA, void* dB, void* dC, float* dD, void* dz,
+                                 float* ddt_bias, float* dinitial) {
+  if (!c) return B200CONV_E_INVALID;
+  std::lock_guard<std::mutex> g(c->mu);
+  DeviceGuard dg(c->device);
+  int rc = check_scan(c, d, x, dt, A, B, C, z, starts);
+  if (rc) return rc;
+  if (!d->C) return 0;
+  const long long n = d->packed ? 1 : d->sequences;
+  const int gn = d->groups * d->N;
+  if ((rc = check_rows(c, "dy", dy, d->dy, n, d->length, d->C)) || (rc = check_rows(c, "dx", dx, d->dx, n, d->length, d->C, true)) ||
+      (rc = check_rows(c, "ddt", ddt, d->ddt, n, d->length, d->C, true)) || (rc = check_rows(c, "dz", dz, d->dz, n, d->length, d->C, true)) ||
+      (rc = check_rows(c, "dB", dB, d->dB, n, d->length, gn, true)) || (rc = check_rows(c, "dC", dC, d->dCm, n, d->length, gn, true)))
+    return rc;
+  if (!dA) return fail(c, B200CONV_E_INVALID, "selective scan gradient without dA");
+  if (!z && dz) return fail(c, B200CONV_E_INVALID, "selective scan gradient with dz but without z");
+  const size_t state_bytes = sizeof(float) * static_cast<size_t>(d->sequences) * d->C * d->N;
+  if (!d->sequences || !d->length) {                // sums over no tokens; the states' gradient passes through
+    CU_OK(c, cudaMemsetAsync(dA, 0, sizeof(float) * d->C * d->N, c->stream));
+    if (dD) CU_OK(c, cudaMemsetAsync(dD, 0, sizeof(float) * d->C, c->stream));
+    if (ddt_bias) CU_OK(c, cudaMemsetAsync(ddt_bias, 0, sizeof(float) * d->C, c->stream));
+    if (dinitial && state_bytes && dinitial != dfinal) {
+      if (dfinal) CU_OK(c, cudaMemcpyAsync(dinitial, dfinal, state_bytes, cudaMemcpyDeviceToDevice, c->stream));
+      else CU_OK(c, cudaMemsetAsync(dinitial, 0, state_bytes, c->stream));
+    }
+    return 0;
+  }
+  if (!dy || !dx || !ddt || !dB || !dC || (z && !dz)) return fail(c, B200CONV_E_INVALID, "selective scan gradient without dy, dx, ddt, dB, dC or dz");
+  Scratch tmp(c);
+  ScanArgs a = {};
+  a.d = *d;
+  a.dy = dy; a.x = x; a.dt = dt; a.A = A; a.B = B; a.C = C; a.D = D; a.z = z; a.dt_bias = dt_bias; a.initial = initial; a.dfinal = dfinal;
+  a.starts = d->packed ? starts : nullptr;
+  a.dx = dx; a.ddt = ddt; a.dA = dA; a.dB = dB; a.dC = dC; a.dD = dD; a.dz = dz; a.ddt_bias = ddt_bias; a.dinitial = dinitial;
+  plan_grad_pieces(&a);
+  const void* after = dfinal;
+  if ((rc = detach_state(c, tmp, &after, dinitial, state_bytes))) return rc;
+  a.dfinal = static_cast<const float*>(after);
+  const size_t kept = static_cast<size_t>(scan_kept(a)) * d->C, slots = scan_state_slots(d->N), pieces = static_cast<size_t>(a.pieces) * d->C;
+  auto get = [&](size_t floats, float** p) { return tmp.get(sizeof(float) * floats, reinterpret_cast<void**>(p)); };
+  if ((rc = get(kept * slots, &a.kept)) || (rc = get(static_cast<size_t>(a.tiles / d->groups) * a.rows * gn * 2, &a.partial_bc)) ||
+      (rc = get(pieces * d->N, &a.partial_a)) || (rc = get(pieces * 2, &a.partial_d)))
+    return rc;
+  if (a.piece < d->length &&
+      ((rc = get(kept, &a.kept_sum)) || (rc = get(pieces * slots, &a.piece_state)) || (rc = get(pieces * slots, &a.piece_back)) ||
+       (rc = get(pieces, &a.piece_sum))))
+    return rc;
+  int launches = 0;
+  KLAUNCH(c, kKScan, launch_scan_grad(a, &launches, c->stream));
+  count_launches(c, launches - 1);
+  return 0;
+}
+
+int b200conv_selective_scan_step(b200conv_ctx* c, const b200conv_scan_desc* d, const void* x, const void* dt, const float* A, const void* B, const void* C,
+                                 const float* D, const void* z, const float* dt_bias, float* state, void* y) {
+  if (!c) return B200CONV_E_INVALID;
+  std::lock_guard<std::mutex> g(c->mu);
+  DeviceGuard dg(c->device);
+  if (d && (d->length != 1 || d->packed)) return fail(c, B200CONV_E_INVALID, "a step takes one token of every sequence");
+  int rc = check_scan(c, d, x, dt, A, B, C, z, nullptr);
+  if (rc || (rc = check_rows(c, "y", y, d->y, d->sequences, 1, d->C, true))) return rc;
+  if (!d->C || !d->sequences) return 0;
+  if (!state || !y) return fail(c, B200CONV_E_INVALID, "selective scan step without state or output");
+  ScanArgs a = {};
+  a.d = *d;
+  a.x = x; a.dt = dt; a.A = A; a.B = B; a.C = C; a.D = D; a.z = z; a.dt_bias = dt_bias; a.final = state; a.y = y;
+  KLAUNCH(c, kKScan, launch_scan_step(a, c->stream));
   return 0;
 }
 

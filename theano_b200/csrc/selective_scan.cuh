@@ -1,0 +1,143 @@
+// What the passes of the selective scan share: pieces of sequences, tiles of tokens in shared memory, lane sums.
+//
+// A channel's N states are spread over P neighbouring lanes, four to a lane (N <= 4 P; states beyond N stay zero), so that a
+// warp holds 32 / P channels.  Sequences may be cut into pieces of `piece` tokens that blocks take independently; what a piece
+// does to a state is h -> exp(A sum of delta) h + (its own result from zero), so pieces are joined by one exponential each.
+#pragma once
+#include <math_constants.h>
+
+#include <type_traits>
+
+#include "internal.h"
+#include "rows.cuh"
+
+namespace b200 {
+
+constexpr int kScanThreads = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 2^v for the decays, whose arguments lie at or below zero: off by 2^-22 of the result, results below 2^-126 are zero.
+__device__ __forceinline__ float exp2_fast(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float softplus(float v) {
+  // log(1 + e^v) = max(v, 0) + log1p(e^-|v|): no overflow, full precision at both ends
+  return fmaxf(v, 0.f) + log1pf(__expf(-fabsf(v)));
+}
+
+// A log2(e).  A decay of minus infinity ends a state in any step of positive size and, like every other, not in one of size zero
+// (as which the tokens behind a piece count).
+__device__ __forceinline__ float scaled_decay(float A) {
+  const float v = A * kLog2e;
+  return v == -CUDART_INF_F ? -3.4e38f : v;
+}
+
+// The tokens of a piece: sequence `seq`, its tokens [from, to) counted from the tensor's row `row0` of that sequence.
+struct Piece {
+  int seq;
+  long long from, to;            // regular: tokens of the sequence; packed: rows of the tensor
+  long long base;                // sequence whose `seq` stride the tensors are addressed with (packed: 0)
+  int first, last;               // pieces of the same sequence, by number
+  bool valid;
+};
+__device__ __forceinline__ Piece piece_of(const ScanArgs& a, int id) {
+  Piece p;
+  if (!a.d.packed) {
+    p.seq = id / a.pieces_per_seq;
+    const int k = id - p.seq * a.pieces_per_seq;
+    p.from = 1LL * k * a.piece;
+    p.to = p.from + a.piece < a.d.length ? p.from + a.piece : a.d.length;
+    p.base = p.seq;
+    p.first = p.seq * a.pieces_per_seq;
+    p.last = p.first + a.pieces_per_seq - 1;
+    p.valid = true;
+    return p;
+  }
+  // Windows of `piece` rows cut the packed tensor; sequence i meets window k in piece i + k: the number grows by one from
+  // a window to the next and from a sequence to the next, so that no two pieces share it (and some stay empty).
+  const int n = static_cast<int>(a.d.sequences);
+  int lo = 0, hi = n;
+  while (lo < hi) {              // the last sequence whose first piece is not behind `id`
+    const int mid = (lo + hi) >> 1;
+    if (start_of(a.starts, mid, a.d.length) / a.piece + mid <= id) lo = mid + 1;
+    else hi = mid;
+  }
+  p.seq = lo - 1;
+  p.base = 0;
+  p.valid = p.seq >= 0;
+  p.from = p.to = 0;
+  p.first = p.last = id;
+  if (!p.valid) return p;
+  const long long s0 = start_of(a.starts, p.seq, a.d.length), s1 = start_of(a.starts, p.seq + 1, a.d.length);
+  const long long k = id - p.seq, w0 = k * a.piece, w1 = w0 + a.piece;
+  p.from = s0 > w0 ? s0 : w0;
+  p.to = s1 < w1 ? s1 : w1;
+  p.first = p.seq + static_cast<int>(s0 / a.piece);
+  p.last = s1 > s0 ? p.seq + static_cast<int>((s1 - 1) / a.piece) : p.first;
+  if (p.to <= p.from) {
+    p.valid = s1 <= s0 && id == p.first;         // an empty sequence: its state passes through
+    p.to = p.from;
+  }
+  return p;
+}
+
+// The channels of a block lie in one group of B and C.
+struct ScanTile { int group, channel, channels; };
+__device__ __forceinline__ ScanTile scan_tile(const ScanArgs& a, int tile, int width) {
+  const int per = a.d.C / a.d.groups, tiles = (per + width - 1) / width;
+  ScanTile t;
+  t.group = tile / tiles;
+  const int c = (tile - t.group * tiles) * width;
+  t.channel = t.group * per + c;
+  t.channels = per - c < width ? per - c : width;
+  return t;
+}
+
+// Partial sums of a piece without tokens.
+template <int P> __device__ __forceinline__ void clear_piece_sums(const ScanArgs& a, int id, const ScanTile& ct) {
+  for (int i = threadIdx.x; i < ct.channels * a.d.N; i += kScanThreads) a.partial_a[(1LL * id * a.d.C + ct.channel) * a.d.N + i] = 0.f;
+  for (int i = threadIdx.x; i < ct.channels; i += kScanThreads)
+    a.partial_d[2LL * id * a.d.C + ct.channel + i] = a.partial_d[(2LL * id + 1) * a.d.C + ct.channel + i] = 0.f;
+}
+
+// Four values per lane, summed over P lanes: lane q of each four holds the sum of value q (P >= 4), every lane
+// with P = 1, 2 returns what it is to store below.
+template <int P> __device__ __forceinline__ float lane_sums(const float (&v)[4]) {
+  const int lane = threadIdx.x & 3;
+  // halves change places: after this a lane keeps two of the four sums, over two lanes
+  const bool hi = lane & 2;
+  float a = hi ? v[2] : v[0], b = hi ? v[3] : v[1];
+  a += __shfl_xor_sync(~0u, hi ? v[0] : v[2], 2);
+  b += __shfl_xor_sync(~0u, hi ? v[1] : v[3], 2);
+  const bool odd = lane & 1;
+  float r = (odd ? b : a) + __shfl_xor_sync(~0u, odd ? a : b, 1);
+#pragma unroll
+  for (int o = 4; o < P; o <<= 1) r += __shfl_xor_sync(~0u, r, o);
+  return r;
+}
+
+// f(type, pieces of V elements, lanes per channel) for the call's data type and state size
+template <typename T, int V, class F> cudaError_t with_lanes(int N, F f) {
+#define B200_LANES(P) if (N <= 4 * P) return f(T(), std::integral_constant<int, (V < kScanThreads / P ? V : kScanThreads / P)>(), std::integral_constant<int, P>());
+  B200_LANES(4) B200_LANES(8) B200_LANES(16) B200_LANES(32)
+#undef B200_LANES
+  return cudaErrorInvalidValue;
+}
+template <class F> cudaError_t with_scan(const ScanArgs& a, bool wide, F f) {
+  if (a.d.dtype == B200CONV_F32) return wide ? with_lanes<float, 4>(a.d.N, f) : with_lanes<float, 1>(a.d.N, f);
+  if (a.d.dtype == B200CONV_F16) return wide ? with_lanes<__half, 8>(a.d.N, f) : with_lanes<__half, 1>(a.d.N, f);
+  return wide ? with_lanes<__nv_bfloat16, 8>(a.d.N, f) : with_lanes<__nv_bfloat16, 1>(a.d.N, f);
+}
+inline int scan_lanes(int N) { return N <= 16 ? 4 : N <= 32 ? 8 : N <= 64 ? 16 : 32; }
+
+// Whether pieces of 16 bytes lie on their boundaries in the tensors of channels, and none straddles two groups.
+inline bool wide_scan(const ScanArgs& a) {
+  const int dt = a.d.dtype, V = dt == B200CONV_F32 ? 4 : 8;
+  return a.d.C / a.d.groups % V == 0 && rows_aligned(a.x, a.d.x, dt) && rows_aligned(a.dt, a.d.dt, dt) && rows_aligned(a.z, a.d.z, dt) &&
+         rows_aligned(a.y, a.d.y, dt) && rows_aligned(a.dy, a.d.dy, dt) && rows_aligned(a.dx, a.d.dx, dt) && rows_aligned(a.ddt, a.d.ddt, dt) &&
+         rows_aligned(a.dz, a.d.dz, dt);
+}
+
+}  // namespace b200

@@ -41,4 +41,28 @@ cudaError_t launch_causal_step(const CausalArgs& a, cudaStream_t s);
 int causal_grad_parts(const CausalArgs& a);
 cudaError_t launch_causal_grad(const CausalArgs& a, int* launches, cudaStream_t s);
 
+// ---- selective scan (selective_scan.cu, selective_scan_grad.cu) ----
+struct ScanArgs {
+  b200conv_scan_desc d;
+  const void *x, *dt, *z, *B, *C, *dy;
+  const float *A, *D, *dt_bias, *initial, *dfinal;
+  const int* starts;
+  void *y, *dx, *ddt, *dz, *dB, *dC;
+  float *final, *dA, *dD, *ddt_bias, *dinitial;
+  // the cut into pieces: tokens of a piece, pieces of a sequence (not of packed ones), of the call; blocks side by side
+  int piece, pieces_per_seq, pieces, tiles;
+  float *piece_state, *piece_sum;          // [pieces][C][4 lanes], [pieces][C]: what a piece makes of zero states, its sum of deltas
+  // gradients: rows of the tensors, the states in front of every eighth token with the sums of deltas up to there, what a piece makes
+  // of a zero adjoint, partial sums: [blocks of a group][rows][groups][2][N], [pieces][C][N], [pieces][2][C]
+  long long rows;
+  float *kept, *kept_sum, *piece_back, *partial_bc, *partial_a, *partial_d;
+};
+void plan_scan_pieces(ScanArgs* a);
+int scan_state_slots(int N);               // states of a channel as the workspaces hold them
+cudaError_t launch_selective_scan(const ScanArgs& a, int* launches, cudaStream_t s);
+void plan_grad_pieces(ScanArgs* a);
+long long scan_kept(const ScanArgs& a);    // kept states per channel
+cudaError_t launch_scan_grad(const ScanArgs& a, int* launches, cudaStream_t s);
+cudaError_t launch_scan_step(const ScanArgs& a, cudaStream_t s);
+
 }  // namespace b200

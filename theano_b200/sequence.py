@@ -475,3 +475,161 @@ def device_causal_conv1d_step(x, state, w, bias=None, silu=False, filter_flip=Tr
     if rc:
         ctx.check(rc)
     return out
+
+
+# ======================================================================================
+# the selective state space scan
+# ======================================================================================
+class ScanDesc(ctypes.Structure):
+    """``b200conv_scan_desc``."""
+    _fields_ = [("sequences", ctypes.c_int64), ("length", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in (
+        "C", "N", "groups", "dtype", "softplus", "packed", "longest", "reserved")] + [
+            (n, Rows) for n in ("x", "dt", "z", "B", "Cm", "y", "dy", "dx", "ddt", "dz", "dB", "dCm")]
+
+
+def _group_rows(what, t, lead):
+    """B or C as (leading axes..., groups, N): its rows, groups and states."""
+    if t is None:
+        return Rows(), None, None
+    if len(t.shape) not in (len(lead) + 1, len(lead) + 2) or t.shape[:len(lead)] != lead:
+        raise ValueError("%s must have shape %s + (groups, states) or (states,), not %s" % (what, lead, t.shape))
+    groups, N = (t.shape[-2] if len(t.shape) == len(lead) + 2 else 1), t.shape[-1]
+    if groups > 1 and N > 0 and t.strides[-2] != N:
+        raise ValueError("the groups of %s must follow each other without gaps" % what)
+    seq, row = (t.strides[0], t.strides[1]) if len(lead) == 2 else (0, t.strides[0])
+    return Rows(row, seq, 0, 0), groups, N
+
+
+def _plan_scan(x, A, vectors, softplus, sequences, states, tensors, grouped):
+    """`tensors`: (field, tensor) like x; `grouped`: (field, tensor) like B; `vectors`: float32 values per channel."""
+    code = _operand_code(x)
+    S, T, C = _batch(x, sequences, "a selective scan")
+    if len(A.shape) != 2 or A.shape[0] != C:
+        raise ValueError("A must have shape (%d, states), not %s" % (C, A.shape))
+    N = A.shape[1]
+    if not 1 <= N <= 128:
+        raise ValueError("a selective scan has 1 to 128 states per channel, not %d" % N)
+    _same("A", A, (C, N), F32)
+    _contiguous("A", A)
+    d = ScanDesc(S, T, C, N, 1, code, int(bool(softplus)), int(sequences is not None), sequences.longest if sequences else 0, 0)
+    d.x = _rows(x)
+    for name, t in tensors:
+        _same(name, t, x.shape, code)
+        if t is not None and t.stored > C:
+            raise ValueError("a selective scan writes no pad channels: %d channels are stored as %d" % (C, t.stored))
+        setattr(d, name, _rows(t))
+    shape = None
+    for name, t in grouped:
+        rows, groups, n = _group_rows(name.replace("Cm", "C"), t, x.shape[:-1])
+        if t is None:
+            continue
+        if t.code != code:
+            raise TypeError("%s must have the tensors' data type" % name.replace("Cm", "C"))
+        shape = shape or (groups, n)
+        if (groups, n) != shape or n != N:
+            raise ValueError("B, C and A disagree about groups or states: %s of %s, A has %d states" % ((groups, n), shape, N))
+        setattr(d, name, rows)
+    d.groups = shape[0]
+    if d.groups < 1 or C % d.groups:
+        raise ValueError("%d channels cannot share %d groups of B and C" % (C, d.groups))
+    for name, t in vectors:
+        _same(name, t, (C,) if not name.endswith("A") else (C, N), F32)
+        _contiguous(name, t)
+    for name, t in states:
+        _same(name, t, (S, C, N), F32)
+        _contiguous(name, t)
+    return ctypes.byref(d)
+
+
+def device_selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=False, initial=None, final=None, sequences=None, out=None):
+    """The selective state space scan over the tokens of every sequence and channel:
+
+        delta = dt + dt_bias (softplus of it);  h = exp(delta * A) * h + delta * x * B;  y = (sum(C * h) + D * x) * (z * sigmoid(z))
+
+    x, dt, z: (sequences, tokens, channels), or (rows, channels) with `sequences`; B, C: the same rows of (groups, states) or
+    (states,), shared by the channels of a group; A (channels, states), D and dt_bias (channels,) float32.  `initial` and `final`:
+    float32 (sequences, channels, states), which may be one array.  Returns `out`, which is none of the inputs."""
+    given, x, dt, A, B, C = x, _array(x), _array(dt), _array(A), _array(B), _array(C)
+    ctx = x.ctx
+    D, z, dt_bias, initial, final = _array(D), _array(z), _array(dt_bias), _array(initial), _array(final)
+    if out is None:
+        out = _like(x, given)
+    y = _array(out)
+    _one_context(ctx, dt, A, B, C, D, z, dt_bias, initial, final, y, sequences)
+    d = _plan(("scan", softplus, x.sig, dt.sig, A.sig, B.sig, C.sig, _sig(D), _sig(z), _sig(dt_bias), _sig(initial), _sig(final), y.sig,
+               _sig(sequences)), lambda: _plan_scan(
+        x, A, (("D", D), ("dt_bias", dt_bias)), softplus, sequences, (("initial", initial), ("final", final)),
+        (("dt", dt), ("z", z), ("y", y)), (("B", B), ("Cm", C))))
+    rc = ctx.lib.b200conv_selective_scan(ctx.h, d, x.ptr, dt.ptr, A.ptr, B.ptr, C.ptr, _ptr(D), _ptr(z), _ptr(dt_bias), _ptr(initial),
+                                         sequences and sequences.starts.ptr, y.ptr, _ptr(final))
+    if rc:
+        ctx.check(rc)
+    return out
+
+
+def device_selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, softplus=False, out=None):
+    """One token of every sequence: x, dt, z (sequences, channels), B, C (sequences, groups, states) or (sequences,
+    states); `state`, float32 (sequences, channels, states), moves on in place.  `out` may be x, dt or z."""
+    x, dt, A, B, C, state = _array(x), _array(dt), _array(A), _array(B), _array(C), _array(state)
+    ctx = x.ctx
+    D, z, dt_bias = _array(D), _array(z), _array(dt_bias)
+    if out is None:
+        out = DeviceArray(ctx, x.shape, x.dtype)
+    y = _array(out)
+    _one_context(ctx, dt, A, B, C, D, z, dt_bias, state, y)
+
+    def make():
+        if len(x.shape) != 2:
+            raise ValueError("a step takes (sequences, channels), not %s" % (x.shape,))
+
+        def token(t):                    # one token per sequence: the sequences' stride is that of the rows
+            return None if t is None else DeviceArray(t.ctx, (t.shape[0], 1) + t.shape[1:], t.dtype, (t.strides[0], t.strides[0]) + t.strides[1:], t.ptr, 0, t)
+        return _plan_scan(token(x), A, (("D", D), ("dt_bias", dt_bias)), softplus, None, (("state", state),),
+                          (("dt", token(dt)), ("z", token(z)), ("y", token(y))), (("B", token(B)), ("Cm", token(C))))
+    d = _plan(("scan step", softplus, x.sig, dt.sig, A.sig, B.sig, C.sig, state.sig, _sig(D), _sig(z), _sig(dt_bias), y.sig), make)
+    rc = ctx.lib.b200conv_selective_scan_step(ctx.h, d, x.ptr, dt.ptr, A.ptr, B.ptr, C.ptr, _ptr(D), _ptr(z), _ptr(dt_bias), state.ptr, y.ptr)
+    if rc:
+        ctx.check(rc)
+    return out
+
+
+def device_selective_scan_grad(dy, x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=False, initial=None, dfinal=None, sequences=None,
+                               grads=None):
+    """Gradients of `device_selective_scan` for dy and, where given, `dfinal`, the gradient of the final states: a dict with
+    x, dt, A, B, C and, where the call has them, D, z, dt_bias and initial.  `grads`: tensors to write them into, of the inputs'
+    shapes and types; those that it lacks are made."""
+    dy, x, dt, A, B, C = _array(dy), _array(x), _array(dt), _array(A), _array(B), _array(C)
+    ctx = x.ctx
+    D, z, dt_bias, initial, dfinal = _array(D), _array(z), _array(dt_bias), _array(initial), _array(dfinal)
+    inputs = dict(x=x, dt=dt, A=A, B=B, C=C, D=D, z=z, dt_bias=dt_bias, initial=initial)
+    grads = dict(grads or {})
+    for name in grads:
+        if name not in inputs:
+            raise ValueError("no input is called %r" % name)
+    if grads.get("initial") is not None and initial is None:
+        _same("the gradient of the initial states", _array(grads["initial"]), (x.shape[0] if sequences is None else sequences.count,) + A.shape, F32)
+    for name, t in inputs.items():
+        if t is not None and grads.get(name) is None:
+            grads[name] = DeviceArray(ctx, t.shape, t.dtype)
+        elif t is None and name != "initial" and grads.get(name) is not None:
+            raise ValueError("the gradient of %s without %s" % (name, name))
+    g = {name: _array(grads.get(name)) for name in inputs}
+    _one_context(ctx, dy, dt, A, B, C, D, z, dt_bias, initial, dfinal, sequences, *g.values())
+
+    def make():
+        for name in ("B", "C"):
+            if g[name].shape != inputs[name].shape:
+                raise ValueError("the gradient of %s must have shape %s, not %s" % (name, inputs[name].shape, g[name].shape))
+        return _plan_scan(x, A, (("D", D), ("dt_bias", dt_bias), ("dA", g["A"]), ("dD", g["D"]), ("ddt_bias", g["dt_bias"])), softplus, sequences,
+                          (("initial", initial), ("dfinal", dfinal), ("dinitial", g["initial"])),
+                          (("dt", dt), ("z", z), ("dy", dy), ("dx", g["x"]), ("ddt", g["dt"]), ("dz", g["z"])),
+                          (("B", B), ("Cm", C), ("dB", g["B"]), ("dCm", g["C"])))
+    d = _plan(("scan grad", softplus, dy.sig, x.sig, dt.sig, A.sig, B.sig, C.sig, _sig(D), _sig(z), _sig(dt_bias), _sig(initial), _sig(dfinal),
+               _sig(sequences)) + tuple(map(_sig, g.values())), make)
+    rc = ctx.lib.b200conv_selective_scan_grad(
+        ctx.h, d, dy.ptr, x.ptr, dt.ptr, A.ptr, B.ptr, C.ptr, _ptr(D), _ptr(z), _ptr(dt_bias), _ptr(initial), _ptr(dfinal),
+        sequences and sequences.starts.ptr, g["x"].ptr, g["dt"].ptr, g["A"].ptr, g["B"].ptr, g["C"].ptr, _ptr(g["D"]), _ptr(g["z"]),
+        _ptr(g["dt_bias"]), _ptr(g["initial"]))
+    if rc:
+        ctx.check(rc)
+    return grads

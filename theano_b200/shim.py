@@ -65,6 +65,9 @@ SIGNATURES = {
     "b200conv_causal_conv": (_I, [_P] * 9),
     "b200conv_causal_conv_grad": (_I, [_P] * 12),
     "b200conv_causal_conv_step": (_I, [_P] * 7),
+    "b200conv_selective_scan": (_I, [_P] * 14),
+    "b200conv_selective_scan_grad": (_I, [_P] * 23),
+    "b200conv_selective_scan_step": (_I, [_P] * 12),
     "b200conv_padded_channels": (_I, [_I, _I]),
     "b200conv_malloc": (_I, [_P, _SZ, ctypes.POINTER(_P)]),
     "b200conv_free": (_I, [_P, _P]),
