@@ -3653,7 +3653,7 @@ int b200conv_selective_scan_grad(b200conv_ctx* c, const b200conv_scan_desc* d, c
   const void* after = dfinal;
   if ((rc = detach_state(c, tmp, &after, dinitial, state_bytes))) return rc;
   a.dfinal = static_cast<const float*>(after);
-  const size_t kept = static_cast<size_t>(scan_kept(a)) * d->C, slots = scan_state_slots(d->N), pieces = static_cast<size_t>(a.pieces) * d->C;
+  const size_t kept = static_cast<size_t>(scan_kept(a)) * d->C, slots = scan_grad_slots(d->N), pieces = static_cast<size_t>(a.pieces) * d->C;
   auto get = [&](size_t floats, float** p) { return tmp.get(sizeof(float) * floats, reinterpret_cast<void**>(p)); };
   if ((rc = get(kept * slots, &a.kept)) || (rc = get(static_cast<size_t>(a.tiles / d->groups) * a.rows * gn * 2, &a.partial_bc)) ||
       (rc = get(pieces * d->N, &a.partial_a)) || (rc = get(pieces * 2, &a.partial_d)))

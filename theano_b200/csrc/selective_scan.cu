@@ -2,145 +2,202 @@
 //
 //   delta = dt + dt_bias (softplus of it),  h[t] = exp(delta A) h[t - 1] + delta x B[t],  y = (sum over n of C[t] h[t] + D x) silu(z)
 //
-// with N states per channel and B, C shared by the channels of a group.  One exponential per token, channel and state:
-// 16 per clock and SM, 4.6e12 a second at 1.965 GHz, which bounds prompts (at N = 16 the tensors' 8 bytes per token and channel
-// take a third of that time).  A block takes 128 / P channels and walks along its tokens in tiles of 32: x, dt and z come
-// in 16-byte pieces that stay in registers, delta and delta x, B and C go through shared memory as float32, the states stay
-// in registers, the sums over the states meet by shuffles four tokens at a time.
+// with N states per channel and B, C shared by the channels of a group.  One exponential per token, channel and state, two where a
+// sequence is cut into pieces: 16 per clock and SM, 4.6e12 a second at 1.965 GHz, which bounds prompts (at N = 16 the tensors' 8
+// bytes per token and channel take a third of that time).  So a lane holds all states of a channel, which makes everything else a
+// token costs (its loads, softplus, gate) as cheap per state as it gets, two states go through the polynomial instead of the special
+// function unit, and the rest runs on packed pairs.  8192 tokens, 2048 channels, 16 states, bfloat16: 191 us in 37 pieces.
 #include "selective_scan.cuh"
 
 namespace b200 {
 namespace {
 
-constexpr int kTile = 32;                        // tokens
-constexpr int kPitch = kTile + 4;                // of a channel's tokens in shared memory
+// A lane per channel (P lanes where there are more than 16 states): S states in registers, so that what a token costs beside the decays
+// is shared by all of them; the rows of B and C, the same for all lanes, come from shared memory as float32.
+constexpr int kScanBlocks = 4;                   // of an SM: 16 warps, 128 registers a thread
+constexpr int kPolyPairs = 1;                    // pairs of decays that a lane takes by polynomial: none 227, one 210, two 216 us (8192 tokens, 2048 channels)
+constexpr int tile_tokens(int NS) { return NS <= 32 ? 32 : 1024 / NS; }           // of a tile of B and C
 
-// Reads a piece's B or C rows into [kTile][4 P] float32, zeros beyond N and beyond the piece.
-template <typename T, int P>
-__device__ __forceinline__ void load_states(const void* src, const b200conv_rows& r, long long base, long long tok, long long to, int group, int N,
-                                            float* dst) {
-  const T* p = static_cast<const T*>(src) + base * r.seq + 1LL * group * N;
-  for (int i = threadIdx.x; i < kTile * 4 * P; i += kScanThreads) {
-    const int t = i / (4 * P), n = i % (4 * P);
-    dst[i] = n < N && tok + t < to ? to_float(p[(tok + t) * r.row + n]) : 0.f;
+// Rows of B (and C) of a tile on their way to shared memory: [B or C][tokens][NS], zeros beyond N and beyond the piece.
+template <typename T, int NS, bool WIDE, bool BOTH>
+struct StateRows {
+  static constexpr int kTokens = tile_tokens(NS), kVec = WIDE ? 16 / sizeof(T) : 1, kRow = NS / kVec, kAll = (BOTH ? 2 : 1) * kTokens * kRow,
+                       kMine = (kAll + kScanThreads - 1) / kScanThreads;
+  Pack<T, kVec> v[kMine];
+  __device__ __forceinline__ void load(const T* B, long long brow, const T* C, long long crow, long long tok, long long to, int N) {
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      const int i = threadIdx.x + k * kScanThreads, which = BOTH ? i / (kTokens * kRow) : 0, t = i / kRow % kTokens, n = i % kRow * kVec;
+      if (i < kAll && tok + t < to && n < N) v[k].load(which ? C + (tok + t) * crow + n : B + (tok + t) * brow + n);
+      else v[k].clear();
+    }
   }
-}
+  __device__ __forceinline__ void store(float* dst) const {
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      const int i = threadIdx.x + k * kScanThreads;
+      if (i >= kAll) break;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) dst[i * kVec + e] = v[k].get(e);
+    }
+  }
+};
 
-// LOCAL: what a piece makes of zero states, and the sum of its deltas; else the outputs, from the states that the pieces before leave.
-template <typename T, int V, int P, bool LOCAL>
-__global__ void __launch_bounds__(kScanThreads) scan_kernel(ScanArgs a) {
-  constexpr int kWide = kScanThreads / P;        // channels of a block
-  constexpr int kParts = (kTile * kWide / V + kScanThreads - 1) / kScanThreads;
+template <typename T, int S, int P, bool WIDE, bool LOCAL>
+__global__ void __launch_bounds__(kScanThreads, S * P <= 32 ? kScanBlocks : 1) scan_lane_kernel(ScanArgs a) {
+  constexpr int NS = S * P, kWide = kScanThreads / P, kTokens = tile_tokens(NS);
+  constexpr int kGroup = LOCAL ? 8 : 4;          // tokens whose x, dt and z a lane has in flight
+  using Rows = StateRows<T, NS, WIDE, !LOCAL>;
   pdl_enter();
-  __shared__ __align__(16) float sd[kWide][kPitch], su[kWide][kPitch], sy[LOCAL ? 1 : kWide][kPitch];
-  __shared__ __align__(16) float sb[kTile * 4 * P], sc[LOCAL ? 1 : kTile * 4 * P];
+  __shared__ __align__(16) float st[2][(LOCAL ? 1 : 2) * kTokens * NS];
   const int id = blockIdx.x / a.tiles;
   const ScanTile ct = scan_tile(a, blockIdx.x - id * a.tiles, kWide);
   const Piece p = piece_of(a, id);
   if (!p.valid || (LOCAL && id == p.last)) return;
-  const int q = threadIdx.x % P, ch = threadIdx.x / P, c = ct.channel + ch;
+  const int q = threadIdx.x % P, ch = threadIdx.x / P, c = ct.channel + ch, N = a.d.N;
   const bool mine = ch < ct.channels;
-  const int N = a.d.N;
-  float A[4], h[4], sum = 0.f;
+  Pair A[S / 2], h[S / 2];
+  {
+    float f[S];
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    const int n = 4 * q + s;
-    A[s] = mine && n < N ? scaled_decay(a.A[1LL * c * N + n]) : 0.f;
-    h[s] = 0.f;
-    if (!LOCAL && a.initial && mine && n < N) h[s] = a.initial[(1LL * p.seq * a.d.C + c) * N + n];
+    for (int s = 0; s < S; ++s) f[s] = mine && q * S + s < N ? scaled_decay(a.A[1LL * c * N + q * S + s]) : 0.f;
+#pragma unroll
+    for (int s = 0; s < S / 2; ++s) A[s] = Pair(f[2 * s], f[2 * s + 1]);
+#pragma unroll
+    for (int s = 0; s < S; ++s) f[s] = !LOCAL && a.initial && mine && q * S + s < N ? a.initial[(1LL * p.seq * a.d.C + c) * N + q * S + s] : 0.f;
+#pragma unroll
+    for (int s = 0; s < S / 2; ++s) h[s] = Pair(f[2 * s], f[2 * s + 1]);
   }
   if (!LOCAL && mine)
+#pragma unroll 4
     for (int j = p.first; j < id; ++j) {         // what the pieces before this one made of it
       const float all = a.piece_sum[1LL * j * a.d.C + c];
-      const float4 f = *reinterpret_cast<const float4*>(a.piece_state + (1LL * j * a.d.C + c) * 4 * P + 4 * q);
-      h[0] = exp2_fast(A[0] * all) * h[0] + f.x;
-      h[1] = exp2_fast(A[1] * all) * h[1] + f.y;
-      h[2] = exp2_fast(A[2] * all) * h[2] + f.z;
-      h[3] = exp2_fast(A[3] * all) * h[3] + f.w;
-    }
-  const T* x = static_cast<const T*>(a.x) + p.base * a.d.x.seq + ct.channel;
-  const T* dt = static_cast<const T*>(a.dt) + p.base * a.d.dt.seq + ct.channel;
-  const T* z = a.z ? static_cast<const T*>(a.z) + p.base * a.d.z.seq + ct.channel : nullptr;
-  T* y = LOCAL ? nullptr : static_cast<T*>(a.y) + p.base * a.d.y.seq + ct.channel;
-  for (long long tok = p.from; tok < p.to; tok += kTile) {
-    Pack<T, V> px[kParts], pz[kParts];
-    __syncthreads();                             // the tile before has been read
+      const float4* f = reinterpret_cast<const float4*>(a.piece_state + (1LL * j * a.d.C + c) * NS + q * S);
 #pragma unroll
-    for (int k = 0; k < kParts; ++k) {
-      const int i = threadIdx.x + k * kScanThreads, t = i / (kWide / V), cc = i % (kWide / V) * V;
-      if (i >= kTile * kWide / V) break;
-      const bool in = tok + t < p.to && cc < ct.channels;
-      Pack<T, V> pd;
-      if (in) {
-        px[k].load(x + (tok + t) * a.d.x.row + cc);
-        pd.load(dt + (tok + t) * a.d.dt.row + cc);
-        if (!LOCAL && z) pz[k].load(z + (tok + t) * a.d.z.row + cc);
+      for (int s = 0; s < S / 4; ++s) {
+        const float4 v = f[s];
+        h[2 * s] = fma2(exp2_pair(mul2(A[2 * s], Pair(all, all))), h[2 * s], Pair(v.x, v.y));
+        h[2 * s + 1] = fma2(exp2_pair(mul2(A[2 * s + 1], Pair(all, all))), h[2 * s + 1], Pair(v.z, v.w));
       }
+    }
+  const float bias = mine && a.dt_bias ? a.dt_bias[c] : 0.f, D = mine && a.D ? a.D[c] : 0.f;
+  // lanes without a channel read the block's last one and write nothing
+  const int cr = mine ? c : ct.channel + ct.channels - 1;
+  const long long xr = a.d.x.row, dr = a.d.dt.row, zr = a.d.z.row, yr = a.d.y.row;
+  const T* x = static_cast<const T*>(a.x) + p.base * a.d.x.seq + p.from * xr + cr;
+  const T* dt = static_cast<const T*>(a.dt) + p.base * a.d.dt.seq + p.from * dr + cr;
+  const T* z = !LOCAL && a.z ? static_cast<const T*>(a.z) + p.base * a.d.z.seq + p.from * zr + cr : nullptr;
+  T* y = LOCAL ? nullptr : static_cast<T*>(a.y) + p.base * a.d.y.seq + p.from * yr + cr;
+  const T* B = static_cast<const T*>(a.B) + p.base * a.d.B.seq + 1LL * ct.group * N;
+  const T* C = static_cast<const T*>(a.C) + p.base * a.d.Cm.seq + 1LL * ct.group * N;
+  T nx[kGroup], nd[kGroup], nz[kGroup];
+  auto fetch = [&](int left) {                   // the next tokens of the piece, of which there are `left`
+    if (left >= kGroup) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float d = 0.f, u = 0.f;
-        if (in) {
-          d = pd.get(e) + (a.dt_bias ? a.dt_bias[ct.channel + cc + e] : 0.f);
-          if (a.d.softplus) d = softplus(d);
-          u = d * px[k].get(e);
+      for (int k = 0; k < kGroup; ++k) {
+        nx[k] = x[k * xr];
+        nd[k] = dt[k * dr];
+        if (z) nz[k] = z[k * zr];
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k)
+        if (k < left) {
+          nx[k] = x[k * xr];
+          nd[k] = dt[k * dr];
+          if (z) nz[k] = z[k * zr];
         }
-        sd[cc + e][t] = d;
-        su[cc + e][t] = u;
-      }
     }
-    load_states<T, P>(a.B, a.d.B, p.base, tok, p.to, ct.group, N, sb);
-    if (!LOCAL) load_states<T, P>(a.C, a.d.Cm, p.base, tok, p.to, ct.group, N, sc);
-    __syncthreads();
-#pragma unroll 2
-    for (int t = 0; t < kTile; t += 4) {
-      const float4 d4 = *reinterpret_cast<const float4*>(&sd[ch][t]), u4 = *reinterpret_cast<const float4*>(&su[ch][t]);
-      const float d[4] = {d4.x, d4.y, d4.z, d4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
-      float out[4];
+    x += kGroup * xr;
+    dt += kGroup * dr;
+    if (z) z += kGroup * zr;
+  };
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float4 b4 = *reinterpret_cast<const float4*>(sb + (t + k) * 4 * P + 4 * q);
-        const float b[4] = {b4.x, b4.y, b4.z, b4.w};
+  for (int k = 0; k < kGroup; ++k) nx[k] = nd[k] = nz[k] = from_float<T>(0.f);
+  Rows rows;
+  rows.load(B, a.d.B.row, C, a.d.Cm.row, p.from, p.to, N);
+  int left = static_cast<int>(p.to - p.from);    // tokens that have not been fetched
+  fetch(left);
+  left -= kGroup;
+  float sum = 0.f;
+  int turn = 0;
+  // kGroup tokens from shared memory at `at`; `live`: how many of them belong to the piece
+  auto group = [&](const float* at, int live, auto whole) {
+    float xv[kGroup], zv[kGroup], d[kGroup], u[kGroup];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) h[s] = exp2_fast(d[k] * A[s]) * h[s] + u[k] * b[s];
-        if (LOCAL) {
-          sum += d[k];
-        } else {
-          const float4 c4 = *reinterpret_cast<const float4*>(sc + (t + k) * 4 * P + 4 * q);
-          out[k] = h[0] * c4.x + h[1] * c4.y + h[2] * c4.z + h[3] * c4.w;
+    for (int k = 0; k < kGroup; ++k) {
+      xv[k] = to_float(nx[k]);
+      if (!LOCAL) zv[k] = to_float(nz[k]);
+      d[k] = to_float(nd[k]) + bias;
+    }
+    if (a.d.softplus)
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k) d[k] = softplus(d[k]);
+#pragma unroll
+    for (int k = 0; k < kGroup; ++k) {
+      if (!decltype(whole)::value && k >= live) d[k] = xv[k] = 0.f;
+      u[k] = d[k] * xv[k];
+      if (LOCAL) sum += d[k];
+    }
+    fetch(left);
+    left -= kGroup;
+#pragma unroll
+    for (int k = 0; k < kGroup; ++k) {
+      const float4* bs = reinterpret_cast<const float4*>(at + k * NS);
+      const float4* cs = LOCAL ? bs : bs + kTokens * NS / 4;
+      const Pair dd(d[k], d[k]), uu(u[k], u[k]);
+      Pair out[2];
+#pragma unroll
+      for (int s = 0; s < S / 4; ++s) {
+        const float4 b = bs[s];
+        const Pair e0 = mul2(dd, A[2 * s]), e1 = mul2(dd, A[2 * s + 1]);
+        h[2 * s] = fma2(2 * s < kPolyPairs ? exp2_poly(e0) : exp2_pair(e0), h[2 * s], mul2(uu, Pair(b.x, b.y)));
+        h[2 * s + 1] = fma2(2 * s + 1 < kPolyPairs ? exp2_poly(e1) : exp2_pair(e1), h[2 * s + 1], mul2(uu, Pair(b.z, b.w)));
+        if (!LOCAL) {
+          const float4 w = cs[s];
+          out[0] = s ? fma2(h[2 * s], Pair(w.x, w.y), out[0]) : mul2(h[0], Pair(w.x, w.y));
+          out[1] = s ? fma2(h[2 * s + 1], Pair(w.z, w.w), out[1]) : mul2(h[1], Pair(w.z, w.w));
         }
       }
-      if (!LOCAL) {
-        const float r = lane_sums<P>(out);
-        if (q < 4) sy[ch][t + q] = r;
-      }
-    }
-    if (LOCAL) continue;
-    __syncthreads();
+      if (LOCAL) continue;
+      const float2 o = add2(out[0], out[1]).get();
+      float r = o.x + o.y;
 #pragma unroll
-    for (int k = 0; k < kParts; ++k) {
-      const int i = threadIdx.x + k * kScanThreads, t = i / (kWide / V), cc = i % (kWide / V) * V;
-      if (i >= kTile * kWide / V || tok + t >= p.to || cc >= ct.channels) break;
-      float out[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        out[e] = sy[cc + e][t];
-        if (a.D) out[e] += a.D[ct.channel + cc + e] * px[k].get(e);
-        if (z) {
-          const float zv = pz[k].get(e);
-          out[e] *= __fdividef(zv, 1.f + __expf(-zv));
-        }
-      }
-      store_row<T, V>(y + (tok + t) * a.d.y.row + cc, out);
+      for (int o = 1; o < P; o <<= 1) r += __shfl_xor_sync(~0u, r, o);
+      r = fmaf(D, xv[k], r);
+      if (z) r *= zv[k] * sigmoid_fast(zv[k]);
+      if (q == 0 && mine && (decltype(whole)::value || k < live)) y[k * yr] = from_float<T>(r);
     }
+    if (!LOCAL) y += kGroup * yr;
+  };
+  for (long long tile = p.from; tile < p.to; tile += kTokens, turn ^= 1) {
+    rows.store(st[turn]);
+    __syncthreads();                             // the tile is there, and the one before the last has been read
+    rows.load(B, a.d.B.row, C, a.d.Cm.row, tile + kTokens, p.to, N);
+    const int n = p.to - tile < kTokens ? static_cast<int>(p.to - tile) : kTokens;
+    const float* at = st[turn] + q * S;
+    int t0 = 0;
+    for (; t0 + kGroup <= n; t0 += kGroup) group(at + t0 * NS, kGroup, std::true_type());
+    if (t0 < n) group(at + t0 * NS, n - t0, std::false_type());
   }
   if (!mine) return;
   if (LOCAL) {
-    *reinterpret_cast<float4*>(a.piece_state + (1LL * id * a.d.C + c) * 4 * P + 4 * q) = make_float4(h[0], h[1], h[2], h[3]);
+    float4* f = reinterpret_cast<float4*>(a.piece_state + (1LL * id * a.d.C + c) * NS + q * S);
+#pragma unroll
+    for (int s = 0; s < S / 4; ++s) {
+      const float2 u = h[2 * s].get(), v = h[2 * s + 1].get();
+      f[s] = make_float4(u.x, u.y, v.x, v.y);
+    }
     if (q == 0) a.piece_sum[1LL * id * a.d.C + c] = sum;
   } else if (a.final && id == p.last) {
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
-      if (4 * q + s < N) a.final[(1LL * p.seq * a.d.C + c) * N + 4 * q + s] = h[s];
+    for (int s = 0; s < S / 2; ++s) {
+      const float2 u = h[s].get();
+      const int n = q * S + 2 * s;
+      float* f = a.final + (1LL * p.seq * a.d.C + c) * N;
+      if (n < N) f[n] = u.x;
+      if (n + 1 < N) f[n + 1] = u.y;
+    }
   }
 }
 
@@ -177,32 +234,42 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(ScanArgs a) {
   if (a.D) y += a.D[c] * x;
   if (a.z) {
     const float z = to_float(static_cast<const T*>(a.z)[seq * a.d.z.seq + c]);
-    y *= __fdividef(z, 1.f + __expf(-z));
+    y *= z * sigmoid_fast(z);
   }
   static_cast<T*>(a.y)[seq * a.d.y.seq + c] = from_float<T>(y);
 }
 
 }  // namespace
 
-cudaError_t launch_selective_scan(const ScanArgs& args, int* launches, cudaStream_t s) {
-  ScanArgs a = args;
-  const int wide = kScanThreads / scan_lanes(a.d.N), per = a.d.C / a.d.groups;
+template <typename T, int S, int P, bool WIDE>
+cudaError_t run_lanes(ScanArgs a, int* launches, cudaStream_t s) {
+  const int wide = kScanThreads / P, per = a.d.C / a.d.groups;
   a.tiles = a.d.groups * ((per + wide - 1) / wide);
   const long long grid = 1LL * a.tiles * a.pieces;
-  *launches = 1;
   if (grid >= INT32_MAX) return cudaErrorInvalidValue;
-  return with_scan(a, wide_scan(a), [&](auto t, auto v, auto p) {
-    using T = decltype(t);
-    constexpr int V = decltype(v)::value, P = decltype(p)::value;
-    if (a.piece_state) {
-      launch_streaming(scan_kernel<T, V, P, true>, static_cast<unsigned>(grid), kScanThreads, 0, s, a);
-      ++*launches;
-      const cudaError_t e = cudaGetLastError();
-      if (e != cudaSuccess) return e;
-    }
-    launch_streaming(scan_kernel<T, V, P, false>, static_cast<unsigned>(grid), kScanThreads, 0, s, a);
-    return cudaGetLastError();
-  });
+  *launches = 1;
+  if (a.piece_state) {
+    launch_streaming(scan_lane_kernel<T, S, P, WIDE, true>, static_cast<unsigned>(grid), kScanThreads, 0, s, a);
+    ++*launches;
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  launch_streaming(scan_lane_kernel<T, S, P, WIDE, false>, static_cast<unsigned>(grid), kScanThreads, 0, s, a);
+  return cudaGetLastError();
+}
+template <typename T>
+cudaError_t run_type(const ScanArgs& a, int* launches, cudaStream_t s) {
+  const int N = a.d.N;
+  const bool wide = N % (16 / sizeof(T)) == 0 && rows_aligned(a.B, a.d.B, a.d.dtype) && rows_aligned(a.C, a.d.Cm, a.d.dtype);
+#define B200_LANES(S, P) if (N <= S * P) return wide ? run_lanes<T, S, P, true>(a, launches, s) : run_lanes<T, S, P, false>(a, launches, s);
+  B200_LANES(8, 1) B200_LANES(16, 1) B200_LANES(16, 2) B200_LANES(16, 4) B200_LANES(16, 8)
+#undef B200_LANES
+  return cudaErrorInvalidValue;
+}
+
+cudaError_t launch_selective_scan(const ScanArgs& a, int* launches, cudaStream_t s) {
+  if (a.d.dtype == B200CONV_F32) return run_type<float>(a, launches, s);
+  return a.d.dtype == B200CONV_F16 ? run_type<__half>(a, launches, s) : run_type<__nv_bfloat16>(a, launches, s);
 }
 
 cudaError_t launch_scan_step(const ScanArgs& a, cudaStream_t s) {
@@ -214,22 +281,22 @@ cudaError_t launch_scan_step(const ScanArgs& a, cudaStream_t s) {
   });
 }
 
-int scan_state_slots(int N) { return 4 * scan_lanes(N); }
+int scan_state_slots(int N) { return N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128; }
 
 // Pieces of a call.  A sequence is cut where its channels alone leave SMs without work: cut, every exponential but those of the last
 // pieces is taken twice.
 void plan_scan_pieces(ScanArgs* a) {
   const long long longest = a->d.packed ? (a->d.longest > 0 && a->d.longest < a->d.length ? a->d.longest : a->d.length) : a->d.length;
-  const int wide = kScanThreads / scan_lanes(a->d.N), per = a->d.C / a->d.groups;
+  const int lanes = a->d.N <= 16 ? 1 : scan_state_slots(a->d.N) / 16, wide = kScanThreads / lanes, per = a->d.C / a->d.groups;
   const long long tiles = 1LL * a->d.groups * ((per + wide - 1) / wide);
   const long long rows = a->d.packed ? a->d.length : a->d.sequences * a->d.length;
   long long piece = a->d.length;
   const long long even = a->d.packed ? (rows + longest - 1) / longest : a->d.sequences;     // sequences that work at the same time to the end
-  if (tiles * even < 148 * 4) {
-    const long long want = (148 * 8 + tiles - 1) / tiles;                                     // pieces of the whole call
+  if (tiles * even < 148 * 2) {
+    const long long want = (148 * kScanBlocks + tiles - 1) / tiles;                                     // pieces of the whole call
     piece = (rows + want - 1) / want;
-    piece = (piece + 63) / 64 * 64;
-    if (piece < 128) piece = 128;
+    piece = (piece + 31) / 32 * 32;
+    if (piece < 32) piece = 32;
   }
   if (piece >= longest) piece = a->d.length > 0 ? a->d.length : 1;
   a->piece = static_cast<int>(piece);

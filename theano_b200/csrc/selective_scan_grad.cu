@@ -451,6 +451,7 @@ __global__ void __launch_bounds__(256) scan_params_kernel(ScanArgs a) {
 
 }  // namespace
 
+int scan_grad_slots(int N) { return 4 * scan_lanes(N); }
 int scan_grad_channels(int N) { return 4 * (kScanThreads / scan_lanes(N)); }
 long long scan_kept(const ScanArgs& a) { return a.rows / kStep + a.pieces + 1; }
 

@@ -61,6 +61,7 @@ void plan_scan_pieces(ScanArgs* a);
 int scan_state_slots(int N);               // states of a channel as the workspaces hold them
 cudaError_t launch_selective_scan(const ScanArgs& a, int* launches, cudaStream_t s);
 void plan_grad_pieces(ScanArgs* a);
+int scan_grad_slots(int N);              // the same in those of the gradient
 long long scan_kept(const ScanArgs& a);    // kept states per channel
 cudaError_t launch_scan_grad(const ScanArgs& a, int* launches, cudaStream_t s);
 cudaError_t launch_scan_step(const ScanArgs& a, cudaStream_t s);
