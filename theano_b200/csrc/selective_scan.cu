@@ -9,39 +9,14 @@
 // function unit, and the rest runs on packed pairs.  8192 tokens, 2048 channels, 16 states, bfloat16: 191 us in 37 pieces.
 #include "selective_scan.cuh"
 
+#include <algorithm>
+
 namespace b200 {
 namespace {
 
 // A lane per channel (P lanes where there are more than 16 states): S states in registers, so that what a token costs beside the decays
 // is shared by all of them; the rows of B and C, the same for all lanes, come from shared memory as float32.
 constexpr int kScanBlocks = 4;                   // of an SM: 16 warps, 128 registers a thread
-constexpr int kPolyPairs = 1;                    // pairs of decays that a lane takes by polynomial: none 227, one 210, two 216 us (8192 tokens, 2048 channels)
-constexpr int tile_tokens(int NS) { return NS <= 32 ? 32 : 1024 / NS; }           // of a tile of B and C
-
-// Rows of B (and C) of a tile on their way to shared memory: [B or C][tokens][NS], zeros beyond N and beyond the piece.
-template <typename T, int NS, bool WIDE, bool BOTH>
-struct StateRows {
-  static constexpr int kTokens = tile_tokens(NS), kVec = WIDE ? 16 / sizeof(T) : 1, kRow = NS / kVec, kAll = (BOTH ? 2 : 1) * kTokens * kRow,
-                       kMine = (kAll + kScanThreads - 1) / kScanThreads;
-  Pack<T, kVec> v[kMine];
-  __device__ __forceinline__ void load(const T* B, long long brow, const T* C, long long crow, long long tok, long long to, int N) {
-#pragma unroll
-    for (int k = 0; k < kMine; ++k) {
-      const int i = threadIdx.x + k * kScanThreads, which = BOTH ? i / (kTokens * kRow) : 0, t = i / kRow % kTokens, n = i % kRow * kVec;
-      if (i < kAll && tok + t < to && n < N) v[k].load(which ? C + (tok + t) * crow + n : B + (tok + t) * brow + n);
-      else v[k].clear();
-    }
-  }
-  __device__ __forceinline__ void store(float* dst) const {
-#pragma unroll
-    for (int k = 0; k < kMine; ++k) {
-      const int i = threadIdx.x + k * kScanThreads;
-      if (i >= kAll) break;
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) dst[i * kVec + e] = v[k].get(e);
-    }
-  }
-};
 
 template <typename T, int S, int P, bool WIDE, bool LOCAL>
 __global__ void __launch_bounds__(kScanThreads, S * P <= 32 ? kScanBlocks : 1) scan_lane_kernel(ScanArgs a) {
@@ -283,25 +258,36 @@ cudaError_t launch_scan_step(const ScanArgs& a, cudaStream_t s) {
 
 int scan_state_slots(int N) { return N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128; }
 
-// Pieces of a call.  A sequence is cut where its channels alone leave SMs without work: cut, every exponential but those of the last
-// pieces is taken twice.
-void plan_scan_pieces(ScanArgs* a) {
-  const long long longest = a->d.packed ? (a->d.longest > 0 && a->d.longest < a->d.length ? a->d.longest : a->d.length) : a->d.length;
-  const int lanes = a->d.N <= 16 ? 1 : scan_state_slots(a->d.N) / 16, wide = kScanThreads / lanes, per = a->d.C / a->d.groups;
-  const long long tiles = 1LL * a->d.groups * ((per + wide - 1) / wide);
-  const long long rows = a->d.packed ? a->d.length : a->d.sequences * a->d.length;
-  long long piece = a->d.length;
-  const long long even = a->d.packed ? (rows + longest - 1) / longest : a->d.sequences;     // sequences that work at the same time to the end
-  if (tiles * even < 148 * 2) {
-    const long long want = (148 * kScanBlocks + tiles - 1) / tiles;                                     // pieces of the whole call
-    piece = (rows + want - 1) / want;
-    piece = (piece + 31) / 32 * 32;
-    if (piece < 32) piece = 32;
+// The cut of a call whose pieces take `tiles` blocks each, on a device that holds `slots` of them at a time: the number of pieces that
+// ends soonest, counted in tokens one after the other, rounds of blocks times a piece's tokens and some for its start.  Half-filled
+// last rounds cost most: 4 sequences of 2048 tokens and 2048 channels, gradients in 4 pieces each on 256 of 296 slots 861 us, in 9
+// pieces in two rounds 752 us.
+void cut_pieces(ScanArgs* a, long long tiles, long long slots) {
+  const long long length = a->d.length, sequences = a->d.sequences, kStart = 24;
+  const long long longest = a->d.packed && a->d.longest > 0 && a->d.longest < length ? a->d.longest : length;
+  long long best = -1, piece = length;
+  for (long long m = 1; m <= 256; ++m) {
+    const long long size = ((longest + m - 1) / m + 3) / 4 * 4;
+    if (m > 1 && size < 32) break;
+    // packed: windows of `size` rows, and a piece more for each sequence that begins inside of one
+    const long long blocks = tiles * (a->d.packed ? length / size + sequences : sequences * ((length + size - 1) / size));
+    // a cut sequence is walked twice, the first time for its ends alone
+    const long long cost = (blocks + slots - 1) / slots * (size + kStart) * (m > 1 ? 7 : 4);
+    if (best < 0 || cost < best) {
+      best = cost;
+      piece = m > 1 ? size : length;
+    }
   }
-  if (piece >= longest) piece = a->d.length > 0 ? a->d.length : 1;
+  piece = std::max<long long>(piece, 1);
   a->piece = static_cast<int>(piece);
-  a->pieces_per_seq = static_cast<int>((a->d.length + piece - 1) / piece);
-  a->pieces = static_cast<int>(a->d.packed ? a->d.sequences + a->d.length / piece : a->d.sequences * a->pieces_per_seq);
+  a->pieces_per_seq = static_cast<int>((length + piece - 1) / piece);
+  a->pieces = static_cast<int>(a->d.packed ? sequences + length / piece : sequences * a->pieces_per_seq);
+}
+
+// Pieces of the forward call: cut, every exponential but those of the last pieces is taken twice.
+void plan_scan_pieces(ScanArgs* a) {
+  const int lanes = a->d.N <= 16 ? 1 : scan_state_slots(a->d.N) / 16, wide = kScanThreads / lanes, per = a->d.C / a->d.groups;
+  cut_pieces(a, 1LL * a->d.groups * ((per + wide - 1) / wide), 148 * kScanBlocks);
 }
 
 }  // namespace b200

@@ -161,9 +161,9 @@ __device__ __forceinline__ ScanTile scan_tile(const ScanArgs& a, int tile, int w
 }
 
 // Partial sums of a piece without tokens.
-template <int P> __device__ __forceinline__ void clear_piece_sums(const ScanArgs& a, int id, const ScanTile& ct) {
-  for (int i = threadIdx.x; i < ct.channels * a.d.N; i += kScanThreads) a.partial_a[(1LL * id * a.d.C + ct.channel) * a.d.N + i] = 0.f;
-  for (int i = threadIdx.x; i < ct.channels; i += kScanThreads)
+__device__ __forceinline__ void clear_piece_sums(const ScanArgs& a, int id, const ScanTile& ct, int threads) {
+  for (int i = threadIdx.x; i < ct.channels * a.d.N; i += threads) a.partial_a[(1LL * id * a.d.C + ct.channel) * a.d.N + i] = 0.f;
+  for (int i = threadIdx.x; i < ct.channels; i += threads)
     a.partial_d[2LL * id * a.d.C + ct.channel + i] = a.partial_d[(2LL * id + 1) * a.d.C + ct.channel + i] = 0.f;
 }
 
@@ -182,6 +182,34 @@ template <int P> __device__ __forceinline__ float lane_sums(const float (&v)[4])
   for (int o = 4; o < P; o <<= 1) r += __shfl_xor_sync(~0u, r, o);
   return r;
 }
+
+constexpr int kPolyPairs = 1;                    // pairs of decays that a lane takes by polynomial: none 227, one 210, two 216 us (8192 tokens, 2048 channels)
+constexpr int tile_tokens(int NS) { return NS <= 32 ? 32 : 1024 / NS; }           // of a tile of B and C
+
+// Rows of B (and C) of a tile on their way to shared memory: [B or C][tokens][NS], zeros beyond N and beyond the piece.
+template <typename T, int NS, bool WIDE, bool BOTH>
+struct StateRows {
+  static constexpr int kTokens = tile_tokens(NS), kVec = WIDE ? 16 / sizeof(T) : 1, kRow = NS / kVec, kAll = (BOTH ? 2 : 1) * kTokens * kRow,
+                       kMine = (kAll + kScanThreads - 1) / kScanThreads;
+  Pack<T, kVec> v[kMine];
+  __device__ __forceinline__ void load(const T* B, long long brow, const T* C, long long crow, long long tok, long long to, int N) {
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      const int i = threadIdx.x + k * kScanThreads, which = BOTH ? i / (kTokens * kRow) : 0, t = i / kRow % kTokens, n = i % kRow * kVec;
+      if (i < kAll && tok + t < to && n < N) v[k].load(which ? C + (tok + t) * crow + n : B + (tok + t) * brow + n);
+      else v[k].clear();
+    }
+  }
+  __device__ __forceinline__ void store(float* dst) const {
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      const int i = threadIdx.x + k * kScanThreads;
+      if (i >= kAll) break;
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) dst[i * kVec + e] = v[k].get(e);
+    }
+  }
+};
 
 // f(type, pieces of V elements, lanes per channel) for the call's data type and state size
 template <typename T, int V, class F> cudaError_t with_lanes(int N, F f) {

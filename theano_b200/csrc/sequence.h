@@ -57,6 +57,7 @@ struct ScanArgs {
   long long rows;
   float *kept, *kept_sum, *piece_back, *partial_bc, *partial_a, *partial_d;
 };
+void cut_pieces(ScanArgs* a, long long tiles, long long slots);
 void plan_scan_pieces(ScanArgs* a);
 int scan_state_slots(int N);               // states of a channel as the workspaces hold them
 cudaError_t launch_selective_scan(const ScanArgs& a, int* launches, cudaStream_t s);
