@@ -8,7 +8,7 @@
 
 namespace b200 {
 
-__device__ __forceinline__ float silu(float v) { return __fdividef(v, 1.f + __expf(-v)); }
+__device__ __forceinline__ float silu(float v) { return v * sigmoid(v); }
 
 // A block is 2^log_lanes channel pieces x 2^(8 - log_lanes) runs; `channel_blocks` blocks side by side span the channels.
 struct CausalGrid {

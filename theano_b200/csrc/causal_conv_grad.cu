@@ -15,7 +15,7 @@ namespace {
 
 // d(pre sigmoid(pre)) = sigmoid (1 + pre (1 - sigmoid))
 __device__ __forceinline__ float silu_slope(float v) {
-  const float s = __fdividef(1.f, 1.f + __expf(-v));
+  const float s = sigmoid(v);
   return s * (1.f + v * (1.f - s));
 }
 
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(512) causal_params_kernel(CausalArgs a, int pa
   if (!out) return;
   float acc = 0.f;
   if (c < C)
-#pragma unroll 4
+#pragma unroll 10
     for (int b = wp; b < parts; b += 16) acc += a.partial[(1LL * b * (K + 1) + k) * C + c];
   part[wp][lane] = acc;
   __syncthreads();

@@ -13,10 +13,11 @@ namespace b200 {
 namespace {
 
 constexpr int kNormThreads = 256;                // of a block, unless a row takes more
-constexpr int kGradThreads = 512;
+constexpr int kGradThreads = 256;
+constexpr int kGradBlocks = 2;                   // of an SM
 
 __device__ __forceinline__ void locate(const b200conv_norm_desc& d, long long row, long long* seq, long long* tok) {
-  if (d.sequences == 1) { *seq = 0; *tok = row; return; }
+  if (d.sequences == 1) { *seq = 0; *tok = row; return; }         // rows that all follow each other
   if (row < (1LL << 31) && d.length < (1LL << 31)) {
     *seq = static_cast<uint32_t>(row) / static_cast<uint32_t>(d.length);
     *tok = row - *seq * d.length;
@@ -43,9 +44,17 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float (*shared)[N]) {
     __syncthreads();
     const int first = warp & ~(TPR / 32 - 1);
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      v[n] = 0.f;
-      for (int w = 0; w < TPR / 32; ++w) v[n] += shared[first + w][n];
+    for (int n = 0; n < N; ++n) v[n] = 0.f;
+    // as wide as the parts lie together: two warps' pairs, four warps' single sums
+    const float4* p = reinterpret_cast<const float4*>(&shared[first][0]);
+#pragma unroll
+    for (int w = 0; w < TPR / 32 * N / 4; ++w) {
+      const float4 f = p[w];
+      if (N == 2) { v[0] += f.x + f.z; v[N - 1] += f.y + f.w; }
+      else v[0] += (f.x + f.y) + (f.z + f.w);
+    }
+    if (TPR / 32 * N < 4) {                      // two warps of single sums
+      v[0] = shared[first][0] + shared[first + 1][0];
     }
   }
 }
@@ -57,10 +66,10 @@ __device__ __forceinline__ void zero_pads(T* row, int C, int stored, int lane, i
 
 // TPR threads per row, VPT pieces of V channels per thread.  C is a multiple of V.
 template <typename T, int V, int VPT, int TPR>
-__global__ void __launch_bounds__(TPR < kNormThreads ? kNormThreads : TPR) norm_kernel(NormArgs a) {
+__global__ void __launch_bounds__(TPR < kNormThreads ? kNormThreads : TPR, VPT >= 4 && TPR < 128 ? 3 : 1) norm_kernel(NormArgs a) {
   constexpr int kThreads = TPR < kNormThreads ? kNormThreads : TPR;
   pdl_enter();
-  __shared__ float part[2][kThreads / 32][1];
+  __shared__ __align__(16) float part[2][kThreads / 32][1];
   const int C = a.d.C, lane = threadIdx.x % TPR;
   const long long rows = a.d.sequences * a.d.length;
   const long long row = 1LL * blockIdx.x * (kThreads / TPR) + threadIdx.x / TPR;
@@ -86,7 +95,7 @@ __global__ void __launch_bounds__(TPR < kNormThreads ? kNormThreads : TPR) norm_
 #pragma unroll
     for (int k = 0; k < VPT; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) px[k].set(i, px[k].get(i) + pr[k].get(i));
+      for (int i = 0; i < kPairs<V>; ++i) put_pair(px[k], i, add2(pair_of(px[k], i, 0.f), pair_of(pr[k], i, 0.f)));
   }
   if (a.total && active) {
     T* t = static_cast<T*>(a.total) + at(a.d.total, seq, tok);
@@ -97,22 +106,25 @@ __global__ void __launch_bounds__(TPR < kNormThreads ? kNormThreads : TPR) norm_
     }
     zero_pads(t, C, a.d.total.stored, lane, TPR);
   }
-  float sum[1] = {0.f};
+  Pair sums(0.f, 0.f);
 #pragma unroll
   for (int k = 0; k < VPT; ++k)
 #pragma unroll
-    for (int i = 0; i < V; ++i) sum[0] += px[k].get(i);
+    for (int i = 0; i < kPairs<V>; ++i) sums = add2(sums, pair_of(px[k], i, 0.f));
+  float sum[1] = {sums.get().x + sums.get().y};
   row_sum<TPR, 1>(sum, part[0]);
   const float mean = sum[0] / C;
-  float sq[1] = {0.f};
+  const Pair away(-mean, -mean);
+  Pair squares(0.f, 0.f);
 #pragma unroll
   for (int k = 0; k < VPT; ++k)
     if ((k * TPR + lane) * V < C)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float d = px[k].get(i) - mean;
-        sq[0] += d * d;
+      for (int i = 0; i < kPairs<V>; ++i) {
+        const Pair d = add2(pair_of(px[k], i, mean), away);
+        squares = fma2(d, d, squares);
       }
+  float sq[1] = {squares.get().x + squares.get().y};
   row_sum<TPR, 1>(sq, part[1]);
   const float rstd = 1.f / sqrtf(sq[0] / C + a.d.eps);
   if (!active) return;
@@ -133,8 +145,13 @@ __global__ void __launch_bounds__(TPR < kNormThreads ? kNormThreads : TPR) norm_
         if (a.gamma) load_params<T, V>(a.gamma, c, gamma);
         if (a.beta) load_params<T, V>(a.beta, c, beta);
       }
+      const Pair scale(rstd, rstd);
 #pragma unroll
-      for (int i = 0; i < V; ++i) o.set(i, (px[k].get(i) - mean) * rstd * gamma[i] + beta[i]);
+      for (int i = 0; i < kPairs<V>; ++i) {
+        constexpr int kNext = V > 1 ? 1 : 0;
+        put_pair(o, i, fma2(mul2(add2(pair_of(px[k], i, mean), away), scale), Pair(gamma[2 * i], gamma[2 * i + kNext]),
+                            Pair(beta[2 * i], beta[2 * i + kNext])));
+      }
       o.store(y + c);
     }
   }
@@ -145,7 +162,7 @@ __global__ void __launch_bounds__(TPR < kNormThreads ? kNormThreads : TPR) norm_
 template <typename T>
 __global__ void __launch_bounds__(512) norm_long_kernel(NormArgs a) {
   pdl_enter();
-  __shared__ float part[2][16][1];
+  __shared__ __align__(16) float part[2][16][1];
   const int C = a.d.C, lane = threadIdx.x;
   long long seq, tok;
   locate(a.d, blockIdx.x, &seq, &tok);
@@ -178,24 +195,29 @@ __global__ void __launch_bounds__(512) norm_long_kernel(NormArgs a) {
 // Backward: blocks stay and walk over the rows, each group of TPR threads with a stride, so that the sums for dgamma and
 // dbeta stay in registers; a block leaves one row of partial sums, which grad_params_kernel adds in block order.
 template <typename T, int V, int VPT, int TPR>
-__global__ void __launch_bounds__(TPR < kGradThreads ? kGradThreads : TPR) norm_grad_kernel(NormArgs a) {
+__global__ void __launch_bounds__(TPR < kGradThreads ? kGradThreads : TPR, TPR <= kGradThreads ? kGradBlocks : 1) norm_grad_kernel(NormArgs a) {
   constexpr int kThreads = TPR < kGradThreads ? kGradThreads : TPR, kGroups = kThreads / TPR;
   pdl_enter();
   extern __shared__ float sums[];                // [kGroups][TPR * VPT * V] of one parameter at a time
-  __shared__ float part[2][kThreads / 32][2];
+  __shared__ __align__(16) float part[2][kThreads / 32][2];
   const int C = a.d.C, lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
   const long long rows = a.d.sequences * a.d.length, step = 1LL * gridDim.x * kGroups;
-  float gamma[VPT][V], dg[VPT][V], db[VPT][V];
+  Pair weight[VPT][kPairs<V>], dg[VPT][kPairs<V>], db[VPT][kPairs<V>];
 #pragma unroll
   for (int k = 0; k < VPT; ++k)
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int c = (k * TPR + lane) * V + i;
-      gamma[k][i] = c >= C ? 0.f : a.gamma ? param<T>(a.gamma, c, a.d.param_f32) : 1.f;
-      dg[k][i] = db[k][i] = 0.f;
+    for (int i = 0; i < kPairs<V>; ++i) {
+      float v[2] = {0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < (V > 1 ? 2 : 1); ++e) {
+        const int c = (k * TPR + lane) * V + 2 * i + e;
+        if (c < C) v[e] = a.gamma ? param<T>(a.gamma, c, a.d.param_f32) : 1.f;
+      }
+      weight[k][i] = Pair(v[0], v[1]);
+      dg[k][i] = db[k][i] = Pair(0.f, 0.f);
     }
-  Pack<T, V> px[VPT], py[VPT];
-  float2 st = make_float2(0.f, 0.f);
+  Pack<T, V> px[VPT], py[VPT], nx[VPT], ny[VPT];
+  float2 st = make_float2(0.f, 0.f), ns = st;
   auto fetch = [&](long long row) {
     if (row >= rows) return;
     long long seq, tok;
@@ -205,34 +227,36 @@ __global__ void __launch_bounds__(TPR < kGradThreads ? kGradThreads : TPR) norm_
 #pragma unroll
     for (int k = 0; k < VPT; ++k) {
       const int c = (k * TPR + lane) * V;
-      if (c < C) { px[k].load(x + c); py[k].load(dy + c); }
+      if (c < C) { nx[k].load(x + c); ny[k].load(dy + c); }
     }
-    st = reinterpret_cast<const float2*>(a.stats)[row];
+    ns = reinterpret_cast<const float2*>(a.stats)[row];
   };
 #pragma unroll
-  for (int k = 0; k < VPT; ++k) { px[k].clear(); py[k].clear(); }
+  for (int k = 0; k < VPT; ++k) { nx[k].clear(); ny[k].clear(); }
   const long long base = 1LL * blockIdx.x * kGroups;
   fetch(base + group);
   int turn = 0;
   for (long long b = base; b < rows; b += step, turn ^= 1) {
     const long long row = b + group;
     const bool active = row < rows;
-    float hat[VPT][V], g[VPT][V], s[2] = {0.f, 0.f};
-    const float rstd = st.y;
+#pragma unroll
+    for (int k = 0; k < VPT; ++k) { px[k] = nx[k]; py[k] = ny[k]; }
+    st = ns;
+    fetch(row + step);                           // the next row is on its way all along
+    const Pair away(-st.x, -st.x), scale(st.y, st.y);
+    Pair g0(0.f, 0.f), g1(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < VPT; ++k)
       if (active && (k * TPR + lane) * V < C)
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float dy = py[k].get(i);
-          hat[k][i] = (px[k].get(i) - st.x) * rstd;
-          g[k][i] = dy * gamma[k][i];
-          dg[k][i] += dy * hat[k][i];
-          db[k][i] += dy;
-          s[0] += g[k][i];
-          s[1] += g[k][i] * hat[k][i];
+        for (int i = 0; i < kPairs<V>; ++i) {
+          const Pair d = pair_of(py[k], i, 0.f), hat = mul2(add2(pair_of(px[k], i, st.x), away), scale), g = mul2(d, weight[k][i]);
+          dg[k][i] = fma2(d, hat, dg[k][i]);
+          db[k][i] = add2(d, db[k][i]);
+          g0 = add2(g, g0);
+          g1 = fma2(g, hat, g1);
         }
-    fetch(row + step);                           // the next row is on its way while this one's sums meet
+    float s[2] = {g0.get().x + g0.get().y, g1.get().x + g1.get().y};
     row_sum<TPR, 2>(s, part[turn]);
     if (!active) continue;
     const float m0 = s[0] / C, m1 = s[1] / C;
@@ -247,8 +271,13 @@ __global__ void __launch_bounds__(TPR < kGradThreads ? kGradThreads : TPR) norm_
         Pack<T, V> o, more;
         if (dt) more.load(dt + c);
         else more.clear();
+        const Pair less(-m0, -m0), slope(-m1, -m1);
 #pragma unroll
-        for (int i = 0; i < V; ++i) o.set(i, rstd * (g[k][i] - m0 - hat[k][i] * m1) + more.get(i));
+        for (int i = 0; i < kPairs<V>; ++i) {
+          const Pair hat = mul2(add2(pair_of(px[k], i, st.x), away), scale);
+          const Pair d = fma2(hat, slope, fma2(pair_of(py[k], i, 0.f), weight[k][i], less));
+          put_pair(o, i, fma2(d, scale, pair_of(more, i, 0.f)));
+        }
         o.store(dx + c);
       }
     }
@@ -264,7 +293,12 @@ __global__ void __launch_bounds__(TPR < kGradThreads ? kGradThreads : TPR) norm_
 #pragma unroll
     for (int k = 0; k < VPT; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) sums[group * kWide + (k * TPR + lane) * V + i] = which ? db[k][i] : dg[k][i];
+      for (int i = 0; i < kPairs<V>; ++i) {
+        const float2 v = (which ? db[k][i] : dg[k][i]).get();
+        float* to = sums + group * kWide + (k * TPR + lane) * V + 2 * i;
+        to[0] = v.x;
+        if (V > 1) to[1] = v.y;
+      }
     __syncthreads();
     for (int c = threadIdx.x; c < C; c += kThreads) {
       float v = 0.f;
@@ -279,7 +313,7 @@ __global__ void __launch_bounds__(TPR < kGradThreads ? kGradThreads : TPR) norm_
 template <typename T>
 __global__ void __launch_bounds__(512) norm_grad_long_kernel(NormArgs a) {
   pdl_enter();
-  __shared__ float part[16][2];
+  __shared__ __align__(16) float part[16][2];
   const int C = a.d.C, lane = threadIdx.x;
   long long seq, tok;
   locate(a.d, blockIdx.x, &seq, &tok);
@@ -334,7 +368,7 @@ __global__ void __launch_bounds__(512) norm_params_kernel(NormArgs a, int parts)
   if (!out) return;
   float acc = 0.f;
   if (c < C)
-#pragma unroll 4
+#pragma unroll 10
     for (int b = wp; b < parts; b += 16) acc += a.partial[(2LL * b + blockIdx.y) * C + c];
   part[wp][lane] = acc;
   __syncthreads();
@@ -360,6 +394,11 @@ cudaError_t forward(const NormArgs& a, cudaStream_t s) {
   }
   if (vecs <= 32) B200_NORM(1, 32)
   if (vecs <= 64) B200_NORM(2, 32)
+  // one or two warps per row; with few rows four warps to a row end sooner
+  if (rows >= 148 * 8) {
+    if (vecs <= 128) B200_NORM(4, 32)
+    if (vecs <= 256) B200_NORM(4, 64)
+  }
   if (vecs <= 128) B200_NORM(1, 128)
   if (vecs <= 256) B200_NORM(2, 128)
   if (vecs <= 512) B200_NORM(4, 128)
@@ -383,10 +422,13 @@ cudaError_t backward(const NormArgs& a, int* launches, cudaStream_t s) {
     break;                                                                                                          \
   }
   do {
+    // two pieces per thread: what a row costs beside its elements (its place, the sums' meeting) is shared by 16 of them; with
+    // one piece and twice the threads 103 us for forward and backward of 16384 x 2048 bfloat16, with two 94, with four 97
     if (vecs <= 32) B200_NORM(1, 32)
-    if (vecs <= 128) B200_NORM(1, 128)
-    if (vecs <= 256) B200_NORM(1, 256)
-    if (vecs <= 512) B200_NORM(1, 512)
+    if (vecs <= 64) B200_NORM(2, 32)
+    if (vecs <= 128) B200_NORM(2, 64)
+    if (vecs <= 256) B200_NORM(2, 128)
+    if (vecs <= 512) B200_NORM(2, 256)
     if (vecs <= 1024) B200_NORM(2, 512)
     launch_streaming(norm_grad_long_kernel<T>, static_cast<unsigned>(rows), 512, 0, s, a);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
@@ -407,7 +449,7 @@ cudaError_t backward(const NormArgs& a, int* launches, cudaStream_t s) {
 // Parts of the parameters' sums: one per block, two blocks per SM once there are rows for them.
 int norm_grad_parts(const b200conv_norm_desc& d) {
   const long long rows = d.sequences * d.length;
-  return static_cast<int>(rows < 1 ? 1 : rows < 148 * 2 ? rows : 148 * 2);
+  return static_cast<int>(rows < 1 ? 1 : rows < 148 * kGradBlocks ? rows : 148 * kGradBlocks);
 }
 
 cudaError_t launch_layer_norm(const NormArgs& args, cudaStream_t s) {

@@ -140,7 +140,7 @@ __global__ void __launch_bounds__(kScanThreads, S * P <= 32 ? kScanBlocks : 1) s
 #pragma unroll
       for (int o = 1; o < P; o <<= 1) r += __shfl_xor_sync(~0u, r, o);
       r = fmaf(D, xv[k], r);
-      if (z) r *= zv[k] * sigmoid_fast(zv[k]);
+      if (z) r *= zv[k] * sigmoid(zv[k]);
       if (q == 0 && mine && (decltype(whole)::value || k < live)) y[k * yr] = from_float<T>(r);
     }
     if (!LOCAL) y += kGroup * yr;
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(kScanThreads) scan_step_kernel(ScanArgs a) {
   if (a.D) y += a.D[c] * x;
   if (a.z) {
     const float z = to_float(static_cast<const T*>(a.z)[seq * a.d.z.seq + c]);
-    y *= z * sigmoid_fast(z);
+    y *= z * sigmoid(z);
   }
   static_cast<T*>(a.y)[seq * a.d.y.seq + c] = from_float<T>(y);
 }

@@ -14,14 +14,7 @@
 namespace b200 {
 
 constexpr int kScanThreads = 128;
-constexpr float kLog2e = 1.4426950408889634f;
 
-// 2^v for the decays, whose arguments lie at or below zero: off by 2^-22 of the result, results below 2^-126 are zero.
-__device__ __forceinline__ float exp2_fast(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
 // log(1 + e^v) = max(v, 0) + log(1 + e) with e = e^-|v| in (0, 1]: no overflow, and full precision for steps near zero.
 // log(1 + e) / e is a polynomial of degree 8 whose coefficients were fitted here by iteratively reweighted least squares (Lawson),
 // off by 3e-8, with float32 roundings by 2e-7: one trip through the special function unit, which the scan's decays already fill.
@@ -37,40 +30,6 @@ __device__ __forceinline__ float softplus(float v) {
   q = fmaf(q, e, -0.4999949336051941f);
   q = fmaf(q, e, 0.9999999403953552f);
   return fmaf(q, e, fmaxf(v, 0.f));
-}
-__device__ __forceinline__ float reciprocal_fast(float v) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-// 1 / (1 + e^-v): zero where e^-v overflows
-__device__ __forceinline__ float sigmoid_fast(float v) { return reciprocal_fast(1.f + exp2_fast(-v * kLog2e)); }
-
-// Two float32 in a 64-bit register: the packed operations take one issue slot for two results.
-struct Pair {
-  unsigned long long v;
-  __device__ __forceinline__ Pair() {}
-  __device__ __forceinline__ Pair(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
-  __device__ __forceinline__ float2 get() const {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-    return f;
-  }
-};
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-  Pair r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-  Pair r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-  Pair r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
 }
 // 2^v of both without the special function unit: v = n + f with n the nearest integer (the low bits of v + 1.5 * 2^23), 2^f a
 // polynomial of degree 5 fitted here by iteratively reweighted least squares (off by 2e-7 with float32 roundings), 2^n into the

@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kScanThreads, S * P <= 32 ? (CUT ? 3 : 4) : 1)
         if (CUT) {
           const float zv = to_float(nz[k]);
           g[k] = to_float(ny[k]);
-          if (z) g[k] *= zv * sigmoid_fast(zv);
+          if (z) g[k] *= zv * sigmoid(zv);
           if (t0 + k >= n) g[k] = 0.f;
         }
       }
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kScanThreads, P == 1 ? kGradBlocks : 1) scan_g
         g[t] = to_float(sh.rows[turn][2][half + t][ch]);
         if (z) {
           const float zv = to_float(sh.rows[turn][3][half + t][ch]);
-          g[t] *= zv * sigmoid_fast(zv);
+          g[t] *= zv * sigmoid(zv);
         }
         if (!in) d[t] = g[t] = xv = 0.f;
         const Pair dd(d[t], d[t]), uu(d[t] * xv, d[t] * xv);
@@ -437,13 +437,13 @@ __global__ void __launch_bounds__(kScanThreads, P == 1 ? kGradBlocks : 1) scan_g
           s3 += __shfl_xor_sync(~0u, s3, k);
         }
         float r = s2 + xv * s1;
-        if (a.d.softplus) r *= sigmoid_fast(to_float(sh.rows[turn][1][half + t][ch]) + bias);
+        if (a.d.softplus) r *= sigmoid(to_float(sh.rows[turn][1][half + t][ch]) + bias);
         if (in && q == 0) {
           const long long at = tok + half + t;
           dx[at * a.d.dx.row] = from_float<T>(d[t] * s1 + D * g[t]);
           ddt[at * a.d.ddt.row] = from_float<T>(r);
           if (dz) {
-            const float zv = to_float(sh.rows[turn][3][half + t][ch]), sg = sigmoid_fast(zv);
+            const float zv = to_float(sh.rows[turn][3][half + t][ch]), sg = sigmoid(zv);
             dz[at * a.d.dz.row] = from_float<T>(to_float(sh.rows[turn][2][half + t][ch]) * (s3 + D * xv) * (sg * (1.f + zv * (1.f - sg))));
           }
           sum_d += g[t] * xv;
