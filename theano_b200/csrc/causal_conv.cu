@@ -14,8 +14,9 @@ namespace {
 
 constexpr int kAhead = 4;                        // rows whose loads a thread has in flight
 
+template <typename T, int K> constexpr int kBlocks = K <= 4 && sizeof(T) == 2 ? 3 : 2;     // of an SM: what the registers allow
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(256) causal_conv_kernel(CausalArgs a, CausalGrid g) {
+__global__ void __launch_bounds__(256, kBlocks<T, K>) causal_conv_kernel(CausalArgs a, CausalGrid g) {
   pdl_enter();
   if (blockIdx.x >= g.run_blocks) {              // the states behind the sequences, in blocks of their own
     final_state<T, V, K>(a, blockIdx.x - g.run_blocks);
@@ -23,50 +24,74 @@ __global__ void __launch_bounds__(256) causal_conv_kernel(CausalArgs a, CausalGr
   }
   const int c = ((blockIdx.x % g.channel_blocks << g.log_lanes) + (threadIdx.x & ((1 << g.log_lanes) - 1))) * V;
   const long long run = (static_cast<long long>(blockIdx.x / g.channel_blocks) << (8 - g.log_lanes)) + (threadIdx.x >> g.log_lanes);
-  if (c >= a.d.C) return;
-  RunPlace p = place_run(a, g, run);
-  if (p.from >= p.to) return;
-  float w[K][V], bias[V];
+  const RunPlace p = place_run(a, g, run);
+  Place at = place_run_start(a, p);
+  if (c >= a.d.C || p.from >= p.to) return;
+  Pair w[K][kPairs<V>], bias[kPairs<V>], win[K - 1][kPairs<V>];
   load_filter<T, V, K>(a, c, w, bias);
+  const long long xr = a.d.x.row, yr = a.d.y.row;
   const T* x = static_cast<const T*>(a.x) + p.seq * a.d.x.seq + c;
   T* y = static_cast<T*>(a.y) + p.seq * a.d.y.seq + c;
-  Place at = place_token(a, p, p.from);
   long long t = at.token;
   if (t >= p.to) return;                         // rows of no sequence
-  float win[K - 1][V];
-  load_window<T, V, K>(a, x, at, t, c, win);
-  while (t < p.to) {
-    Pack<T, V> in[kAhead];
+  Pack<T, V> in[kAhead], next[kAhead];
+  auto fetch = [&](const T* from, int left, Pack<T, V> (&to)[kAhead]) {
+    if (left >= kAhead) {
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if (t + k < p.to) in[k].load(x + (t + k) * a.d.x.row);
+      for (int k = 0; k < kAhead; ++k) to[k].load(from + k * xr);
+    } else {
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      if (t + k >= p.to) break;
-      if (t + k >= at.end) {                     // packed sequences: the next one begins here, or rows of none
-        if (!next_sequence(a, t + k, &at)) return;
-        if (at.token == t + k) load_window<T, V, K>(a, x, at, t + k, c, win);
-      }
-      float now[V], out[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        now[i] = in[k].get(i);
-        float pre = bias[i] + w[0][i] * now[i];
-#pragma unroll
-        for (int j = 1; j < K; ++j) pre += w[j][i] * win[K - 1 - j][i];
-        out[i] = a.d.silu ? silu(pre) : pre;
-      }
-#pragma unroll
-      for (int j = 0; j + 2 < K; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) win[j][i] = win[j + 1][i];
-#pragma unroll
-      for (int i = 0; i < V; ++i) win[K - 2][i] = now[i];
-      store_row<T, V>(y + (t + k) * a.d.y.row, out);
-      if (c + V >= a.d.C)
-        for (int z = V; c + z < a.d.y.stored; ++z) y[(t + k) * a.d.y.row + z] = from_float<T>(0.f);
+      for (int k = 0; k < kAhead; ++k)
+        if (k < left) to[k].load(from + k * xr);
     }
+  };
+  const T* from = x + t * xr;
+  T* to = y + t * yr;
+  int left = static_cast<int>(p.to - t), same = static_cast<int>((at.end < p.to ? at.end : p.to) - t);      // tokens of the run, of this sequence in it
+  fetch(from, left, in);
+  load_window<T, V, K>(a, x, at, t, c, win);
+  const bool pads = c + V >= a.d.C && a.d.y.stored > a.d.C;
+  auto token = [&](int k) {
+    Pack<T, V> o;
+#pragma unroll
+    for (int i = 0; i < kPairs<V>; ++i) {
+      const Pair now = pair_of(in[k], i, 0.f);
+      Pair pre = fma2(w[0][i], now, bias[i]);
+#pragma unroll
+      for (int j = 1; j < K; ++j) pre = fma2(w[j][i], win[K - 1 - j][i], pre);
+      put_pair(o, i, a.d.silu ? silu2(pre) : pre);
+#pragma unroll
+      for (int j = 0; j + 2 < K; ++j) win[j][i] = win[j + 1][i];
+      win[K - 2][i] = now;
+    }
+    o.store(to + k * yr);
+    if (pads)
+      for (int z = V; c + z < a.d.y.stored; ++z) to[k * yr + z] = from_float<T>(0.f);
+  };
+  while (left > 0) {
+    from += kAhead * xr;
+    fetch(from, left - kAhead, next);            // on their way while these are computed
+    if (same >= kAhead) {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) token(k);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        if (k >= left) break;
+        if (k >= same) {                         // packed sequences: the next one begins here, or rows of none
+          if (!next_sequence(a, t + k, &at)) return;
+          load_window<T, V, K>(a, x, at, t + k, c, win);
+          same = static_cast<int>((at.end < p.to ? at.end : p.to) - t);
+        }
+        token(k);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) in[k] = next[k];
     t += kAhead;
+    left -= kAhead;
+    same -= kAhead;
+    to += kAhead * yr;
   }
 }
 
@@ -87,9 +112,9 @@ __global__ void __launch_bounds__(128) causal_step_kernel(CausalArgs a, int vecs
   load_filter<T, V, K>(a, c, w, bias);
 #pragma unroll
   for (int q = 0; q < V; ++q) {
-    float pre = bias[q] + w[0][q] * now.get(q);
+    float pre = fmaf(w[0][q], now.get(q), bias[q]);       // in the order of a prompt
 #pragma unroll
-    for (int j = 1; j < K; ++j) pre += w[j][q] * old[K - 1 - j].get(q);
+    for (int j = 1; j < K; ++j) pre = fmaf(w[j][q], old[K - 1 - j].get(q), pre);
     out[q] = a.d.silu ? silu(pre) : pre;
   }
 #pragma unroll
@@ -103,7 +128,7 @@ __global__ void __launch_bounds__(128) causal_step_kernel(CausalArgs a, int vecs
 
 template <typename T, int V, int K>
 cudaError_t forward(const CausalArgs& a, cudaStream_t s) {
-  const CausalGrid g = causal_grid(a, V, 148 * 2048, kAhead, 32);
+  const CausalGrid g = causal_grid(a, V, 256, 148 * kBlocks<T, K>, kAhead);
   long long grid = g.run_blocks;
   if (a.final) grid += (a.d.sequences * (K - 1) * (a.d.C / V) + 255) / 256;
   if (grid >= INT32_MAX) return cudaErrorInvalidValue;
@@ -122,7 +147,7 @@ cudaError_t step(const CausalArgs& a, cudaStream_t s) {
 }  // namespace
 
 cudaError_t launch_causal_conv(const CausalArgs& a, cudaStream_t s) {
-  return with_causal(a, wide_causal(a), [&](auto t, auto v, auto k) { return forward<decltype(t), decltype(v)::value, decltype(k)::value>(a, s); });
+  return with_causal<4>(a, wide_causal(a), [&](auto t, auto v, auto k) { return forward<decltype(t), decltype(v)::value, decltype(k)::value>(a, s); });
 }
 cudaError_t launch_causal_step(const CausalArgs& a, cudaStream_t s) {
   return with_causal(a, wide_causal(a), [&](auto t, auto v, auto k) { return step<decltype(t), decltype(v)::value, decltype(k)::value>(a, s); });

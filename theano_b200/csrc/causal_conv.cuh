@@ -10,24 +10,26 @@ namespace b200 {
 
 __device__ __forceinline__ float silu(float v) { return v * sigmoid(v); }
 
-// A block is 2^log_lanes channel pieces x 2^(8 - log_lanes) runs; `channel_blocks` blocks side by side span the channels.
+// A block is 2^log_lanes (32 or 64) channel pieces x threads >> log_lanes runs; `channel_blocks` blocks side by side span the channels.
 struct CausalGrid {
-  int log_lanes, channel_blocks;
+  int threads, log_lanes, channel_blocks;
   int run;                                       // tokens of a run
   int runs;                                      // runs of a sequence (packed: of the tensor)
   unsigned run_blocks;
 };
-inline CausalGrid causal_grid(const CausalArgs& a, int V, long long threads, int least, int most) {
+// Runs as long as lets all blocks be resident at once (`slots` of them), `least` tokens at least: a few blocks more than fit would be a
+// second round, and every run costs its filters and the tokens before it.
+inline CausalGrid causal_grid(const CausalArgs& a, int V, int threads, long long slots, int least) {
   CausalGrid g = {};
-  const long long vecs = a.d.C / V, rows = a.d.packed ? a.d.length : a.d.sequences * a.d.length;
-  while (g.log_lanes < 8 && (1LL << g.log_lanes) < vecs) ++g.log_lanes;
-  if (g.log_lanes > 6) g.log_lanes = 6;          // 64 pieces are 1 KB side by side; the other threads take the runs next to it
+  const long long vecs = a.d.C / V, sequences = a.d.packed ? 1 : a.d.sequences;
+  g.threads = threads;
+  g.log_lanes = 5;                               // a warp works on one run
+  while (g.log_lanes < 6 && (1LL << g.log_lanes) < vecs) ++g.log_lanes;
   g.channel_blocks = static_cast<int>((vecs + (1LL << g.log_lanes) - 1) >> g.log_lanes);
-  const long long want = (rows * vecs + threads - 1) / threads;
-  g.run = static_cast<int>(std::min<long long>(std::max<long long>(want, least), most));
+  const long long per = threads >> g.log_lanes, at_once = std::max<long long>(1, slots / g.channel_blocks * per / std::max<long long>(1, sequences));
+  g.run = static_cast<int>(std::max<long long>((a.d.length + at_once - 1) / at_once, least));
   g.runs = static_cast<int>((a.d.length + g.run - 1) / g.run);
-  const long long all = a.d.packed ? g.runs : a.d.sequences * g.runs, per = 1LL << (8 - g.log_lanes);
-  g.run_blocks = static_cast<unsigned>((all + per - 1) / per * g.channel_blocks);
+  g.run_blocks = static_cast<unsigned>((sequences * g.runs + per - 1) / per * g.channel_blocks);
   return g;
 }
 
@@ -43,18 +45,13 @@ __device__ __forceinline__ RunPlace place_run(const CausalArgs& a, const CausalG
 
 // The sequence that a token belongs to, and the first token of the run that belongs to any.
 struct Place { int seq; long long begin, end, token; };
-__device__ __forceinline__ Place place_token(const CausalArgs& a, const RunPlace& p, long long t) {
+// From sequence `seq` on, past empty ones and rows in front of the first.
+__device__ __forceinline__ Place place_from(const CausalArgs& a, int seq, long long t) {
   Place at;
-  if (!a.d.packed) {
-    at.seq = static_cast<int>(p.seq);
-    at.begin = 0; at.end = a.d.length; at.token = t;
-    return at;
-  }
   const int n = static_cast<int>(a.d.sequences);
-  at.seq = sequence_of(a.starts, n, t, a.d.length);
-  if (at.seq < 0) at.seq = 0;
-  at.token = a.d.length;
-  for (; at.seq < n; ++at.seq) {                 // past empty sequences, and rows in front of the first
+  at.seq = seq < 0 ? 0 : seq;
+  at.begin = at.end = at.token = a.d.length;
+  for (; at.seq < n; ++at.seq) {
     at.begin = start_of(a.starts, at.seq, a.d.length);
     at.end = start_of(a.starts, at.seq + 1, a.d.length);
     const long long first = at.begin > t ? at.begin : t;
@@ -62,11 +59,18 @@ __device__ __forceinline__ Place place_token(const CausalArgs& a, const RunPlace
   }
   return at;
 }
+// The place of a run's first token (all lanes of a warp call this, for the same run).
+__device__ __forceinline__ Place place_run_start(const CausalArgs& a, const RunPlace& p) {
+  if (a.d.packed) return place_from(a, sequence_of(a.starts, static_cast<int>(a.d.sequences), p.from, a.d.length), p.from);
+  Place at;
+  at.seq = static_cast<int>(p.seq);
+  at.begin = 0; at.end = a.d.length; at.token = p.from;
+  return at;
+}
 // Token t lies behind at's sequence: the one that it belongs to.  False where no later row belongs to any.
 __device__ __forceinline__ bool next_sequence(const CausalArgs& a, long long t, Place* at) {
   if (!a.d.packed) return false;
-  const RunPlace none = {0, 0, 0};
-  *at = place_token(a, none, t);
+  *at = place_from(a, at->seq + 1, t);
   return at->token == t;
 }
 
@@ -100,6 +104,27 @@ __device__ __forceinline__ void load_filter(const CausalArgs& a, int c, float (&
     for (int q = 0; q < V; ++q) w[k][q] = a.d.flip ? flat[q * K + k] : flat[q * K + K - 1 - k];
 }
 
+// Coefficients and bias in pairs of channels.
+template <typename T, int V, int K>
+__device__ __forceinline__ void load_filter(const CausalArgs& a, int c, Pair (&w)[K][kPairs<V>], Pair (&bias)[kPairs<V>]) {
+  constexpr int kNext = V > 1 ? 1 : 0;
+  float fw[K][V], fb[V];
+  load_filter<T, V, K>(a, c, fw, fb);
+#pragma unroll
+  for (int i = 0; i < kPairs<V>; ++i) {
+    bias[i] = Pair(fb[2 * i], fb[2 * i + kNext]);
+#pragma unroll
+    for (int k = 0; k < K; ++k) w[k][i] = Pair(fw[k][2 * i], fw[k][2 * i + kNext]);
+  }
+}
+
+// v sigmoid(v) of both
+__device__ __forceinline__ Pair silu2(Pair v) {
+  const float2 e = mul2(v, Pair(-kLog2e, -kLog2e)).get();
+  const float2 d = add2(Pair(exp2_fast(e.x), exp2_fast(e.y)), Pair(1.f, 1.f)).get();
+  return mul2(v, Pair(reciprocal_fast(d.x), reciprocal_fast(d.y)));
+}
+
 // The taps - 1 rows before token t of at's sequence, oldest first: tokens, rows of the initial state, zeros.
 template <typename T, int V, int K>
 __device__ __forceinline__ void load_window(const CausalArgs& a, const T* x, const Place& at, long long t, int c, float (&win)[K - 1][V]) {
@@ -112,6 +137,17 @@ __device__ __forceinline__ void load_window(const CausalArgs& a, const T* x, con
 #pragma unroll
       for (int i = 0; i < V; ++i) win[j][i] = 0.f;
   }
+}
+
+template <typename T, int V, int K>
+__device__ __forceinline__ void load_window(const CausalArgs& a, const T* x, const Place& at, long long t, int c, Pair (&win)[K - 1][kPairs<V>]) {
+  constexpr int kNext = V > 1 ? 1 : 0;
+  float f[K - 1][V];
+  load_window<T, V, K>(a, x, at, t, c, f);
+#pragma unroll
+  for (int j = 0; j < K - 1; ++j)
+#pragma unroll
+    for (int i = 0; i < kPairs<V>; ++i) win[j][i] = Pair(f[j][2 * i], f[j][2 * i + kNext]);
 }
 
 // Rows of the final states: thread i of these blocks takes one piece of one row of one sequence.

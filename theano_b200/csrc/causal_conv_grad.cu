@@ -23,7 +23,7 @@ __device__ __forceinline__ float silu_slope(float v) {
 template <typename T, int V, int K>
 __device__ void initial_grad(const CausalArgs& a, long long block) {
   const int vecs = a.d.C / V;
-  const long long i = block * 256 + threadIdx.x;
+  const long long i = block * blockDim.x + threadIdx.x;
   if (i >= a.d.sequences * (K - 1) * vecs) return;
   const int c = static_cast<int>(i % vecs) * V, j = static_cast<int>(i / vecs % (K - 1));
   Place at;
@@ -56,89 +56,122 @@ __device__ void initial_grad(const CausalArgs& a, long long block) {
   store_row<T, V>(static_cast<T*>(a.dinitial) + ((K - 1LL) * at.seq + j) * a.d.C + c, sum);
 }
 
+// The slope of both
+__device__ __forceinline__ Pair silu_slope2(Pair v) {
+  const float2 e = mul2(v, Pair(-kLog2e, -kLog2e)).get();
+  const Pair one(1.f, 1.f);
+  const float2 d = add2(Pair(exp2_fast(e.x), exp2_fast(e.y)), one).get();
+  const Pair s(reciprocal_fast(d.x), reciprocal_fast(d.y));
+  return mul2(s, fma2(v, fma2(s, Pair(-1.f, -1.f), one), one));
+}
+
+constexpr int kGradThreads = 128;
+template <int K> constexpr int kGradBlocks = K <= 4 ? 3 : 2;            // of an SM
+
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(256) causal_grad_kernel(CausalArgs a, CausalGrid g) {
+__global__ void __launch_bounds__(kGradThreads, kGradBlocks<K>) causal_grad_kernel(CausalArgs a, CausalGrid g) {
+  constexpr int H = kPairs<V>;
   pdl_enter();
-  __shared__ float part[256][V + 1];
+  __shared__ float part[kGradThreads][V + 1];
   if (blockIdx.x >= g.run_blocks) {
     initial_grad<T, V, K>(a, blockIdx.x - g.run_blocks);
     return;
   }
-  const int lanes = 1 << g.log_lanes, lane = threadIdx.x & (lanes - 1);
+  const int lanes = 1 << g.log_lanes, lane = threadIdx.x & (lanes - 1), rows = kGradThreads >> g.log_lanes;
   const int cb = blockIdx.x % g.channel_blocks, rb = blockIdx.x / g.channel_blocks;
   const int c = ((cb << g.log_lanes) + lane) * V;
   const bool inside = c < a.d.C;
-  RunPlace p = place_run(a, g, (static_cast<long long>(rb) << (8 - g.log_lanes)) + (threadIdx.x >> g.log_lanes));
-  float w[K][V], bias[V], dw[K][V], db[V];
+  const RunPlace p = place_run(a, g, 1LL * rb * rows + (threadIdx.x >> g.log_lanes));
+  Place at = place_run_start(a, p);
+  Pair dw[K][H], db[H];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    db[i] = 0.f;
+  for (int i = 0; i < H; ++i) {
+    db[i] = Pair(0.f, 0.f);
 #pragma unroll
-    for (int k = 0; k < K; ++k) dw[k][i] = 0.f;
+    for (int k = 0; k < K; ++k) dw[k][i] = Pair(0.f, 0.f);
   }
   if (inside && p.from < p.to) {
+    Pair w[K][H], bias[H];
     load_filter<T, V, K>(a, c, w, bias);
+    const long long xr = a.d.x.row, yr = a.d.dy.row, dr = a.d.dx.row;
     const T* x = static_cast<const T*>(a.x) + p.seq * a.d.x.seq + c;
     const T* dy = static_cast<const T*>(a.dy) + p.seq * a.d.dy.seq + c;
     T* dx = static_cast<T*>(a.dx) + p.seq * a.d.dx.seq + c;
+    const bool pads = c + V >= a.d.C && a.d.dx.stored > a.d.C;
     for (long long from = p.from; from < p.to;) {            // the piece of each sequence in the run
-      const Place at = place_token(a, p, from);
+      if (from > p.from && !next_sequence(a, from, &at)) break;
       from = at.token;
       if (from >= p.to) break;
-      const long long to = at.end < p.to ? at.end : p.to, last = to + K - 1;
-      float win[K - 1][V], acc[K][V];
+      const long long to = at.end < p.to ? at.end : p.to;
+      // tokens of the piece, tokens to read (those beyond it for the sums that end there), rounds until the last sum has left
+      const int mine = static_cast<int>(to - from), read = static_cast<int>((at.end < to + K - 1 ? at.end : to + K - 1) - from), last = mine + K - 1;
+      Pair win[K - 1][H], acc[K - 1][H];
       load_window<T, V, K>(a, x, at, from, c, win);
 #pragma unroll
-      for (int k = 0; k < K; ++k)
+      for (int k = 0; k + 1 < K; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[k][i] = 0.f;
-      constexpr int kStep = 4;
-      for (long long t0 = from; t0 < last; t0 += kStep) {
-        Pack<T, V> px[kStep], pd[kStep];
+        for (int i = 0; i < H; ++i) acc[k][i] = Pair(0.f, 0.f);
+      constexpr int kRound = 4;                  // rows on their way
+      const T* px = x + from * xr;
+      const T* py = dy + from * yr;
+      T* pd = dx + (from - (K - 1)) * dr;
+      Pack<T, V> nx[kRound], ny[kRound], cx[kRound], cy[kRound];
+      auto fetch = [&](int left) {
 #pragma unroll
-        for (int u = 0; u < kStep; ++u) {
-          if (t0 + u < last && t0 + u < at.end) {
-            px[u].load(x + (t0 + u) * a.d.x.row);
-            pd[u].load(dy + (t0 + u) * a.d.dy.row);
-          } else {
-            px[u].clear();
-            pd[u].clear();
+        for (int u = 0; u < kRound; ++u) {
+          nx[u].clear();
+          ny[u].clear();
+          if (u < left) {
+            nx[u].load(px + u * xr);
+            ny[u].load(py + u * yr);
           }
         }
+        px += kRound * xr;
+        py += kRound * yr;
+      };
+      fetch(read);
+      for (int t0 = 0; t0 < last; t0 += kRound) {
 #pragma unroll
-        for (int u = 0; u < kStep; ++u) {
-          const long long t = t0 + u;
+        for (int u = 0; u < kRound; ++u) { cx[u] = nx[u]; cy[u] = ny[u]; }
+        fetch(read - t0 - kRound);               // on their way while these are computed
+#pragma unroll
+        for (int u = 0; u < kRound; ++u) {
+          const int t = t0 + u;
           if (t >= last) break;
-          float done[V];
+          Pack<T, V> done;
+          const bool behind = t >= read, sums = t < mine;
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float now = px[u].get(i);
-            float pre = bias[i] + w[0][i] * now;
+          for (int i = 0; i < H; ++i) {
+            const Pair now = pair_of(cx[u], i, 0.f);
+            Pair gr = pair_of(cy[u], i, 0.f);
+            if (a.d.silu) {
+              Pair pre = fma2(w[0][i], now, bias[i]);
 #pragma unroll
-            for (int k = 1; k < K; ++k) pre += w[k][i] * win[K - 1 - k][i];
-            float gr = pd[u].get(i);
-            if (a.d.silu) gr *= silu_slope(pre);
-            if (t >= at.end) gr = 0.f;                       // behind the sequence: only sums that wait for their store
-            if (t < to) {
-              db[i] += gr;
-              dw[0][i] += gr * now;
-#pragma unroll
-              for (int k = 1; k < K; ++k) dw[k][i] += gr * win[K - 1 - k][i];
+              for (int k = 1; k < K; ++k) pre = fma2(w[k][i], win[K - 1 - k][i], pre);
+              gr = mul2(gr, silu_slope2(pre));
             }
-            done[i] = acc[K - 1][i] + w[K - 1][i] * gr;
+            if (behind) gr = Pair(0.f, 0.f);                 // behind the sequence: only sums that wait for their store
+            if (sums) {
+              db[i] = add2(gr, db[i]);
+              dw[0][i] = fma2(gr, now, dw[0][i]);
 #pragma unroll
-            for (int k = K - 1; k > 0; --k) acc[k][i] = acc[k - 1][i] + w[k - 1][i] * gr;
+              for (int k = 1; k < K; ++k) dw[k][i] = fma2(gr, win[K - 1 - k][i], dw[k][i]);
+            }
+            put_pair(done, i, fma2(w[K - 1][i], gr, acc[K - 2][i]));
+#pragma unroll
+            for (int k = K - 2; k > 0; --k) acc[k][i] = fma2(w[k][i], gr, acc[k - 1][i]);
+            acc[0][i] = mul2(w[0][i], gr);
 #pragma unroll
             for (int j = 0; j + 2 < K; ++j) win[j][i] = win[j + 1][i];
             win[K - 2][i] = now;
           }
-          const long long at_row = t - (K - 1);
-          if (at_row >= from) {
-            store_row<T, V>(dx + at_row * a.d.dx.row, done);
-            if (c + V >= a.d.C)
-              for (int z = V; c + z < a.d.dx.stored; ++z) dx[at_row * a.d.dx.row + z] = from_float<T>(0.f);
+          if (t >= K - 1) {
+            done.store(pd + u * dr);
+            if (pads)
+              for (int z = V; c + z < a.d.dx.stored; ++z) pd[u * dr + z] = from_float<T>(0.f);
           }
         }
+        pd += kRound * dr;
       }
       from = to;
     }
@@ -149,12 +182,16 @@ __global__ void __launch_bounds__(256) causal_grad_kernel(CausalArgs a, CausalGr
 #pragma unroll
   for (int k = 0; k <= K; ++k) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) part[threadIdx.x][i] = k < K ? dw[k < K ? k : 0][i] : db[i];
+    for (int i = 0; i < H; ++i) {
+      const float2 v = (k < K ? dw[k < K ? k : 0][i] : db[i]).get();
+      part[threadIdx.x][2 * i] = v.x;
+      if (V > 1) part[threadIdx.x][2 * i + (V > 1 ? 1 : 0)] = v.y;
+    }
     __syncthreads();
-    for (int e = threadIdx.x; e < lanes * V; e += 256) {
+    for (int e = threadIdx.x; e < lanes * V; e += kGradThreads) {
       const int l = e / V, i = e % V, ch = ((cb << g.log_lanes) + l) * V + i;
       float v = 0.f;
-      for (int r = 0; r < 256 >> g.log_lanes; ++r) v += part[(r << g.log_lanes) + l][i];
+      for (int r = 0; r < rows; ++r) v += part[(r << g.log_lanes) + l][i];
       if (ch < a.d.C) out[1LL * k * a.d.C + ch] = v;
     }
     __syncthreads();
@@ -181,17 +218,18 @@ __global__ void __launch_bounds__(512) causal_params_kernel(CausalArgs a, int pa
   }
 }
 
-// Runs that are long enough for few partial sums, short enough to occupy the SMs with two blocks each.
-CausalGrid grad_grid(const CausalArgs& a, int V) { return causal_grid(a, V, 148 * 2 * 256, 16, 1 << 20); }
+CausalGrid grad_grid(const CausalArgs& a, int V) {
+  return causal_grid(a, V, kGradThreads, 148LL * (a.d.width <= 4 ? kGradBlocks<4> : kGradBlocks<8>), 8);
+}
 
 template <typename T, int V, int K>
 cudaError_t backward(const CausalArgs& a, int* launches, cudaStream_t s) {
   const CausalGrid g = grad_grid(a, V);
   long long grid = g.run_blocks;
-  if (a.dinitial) grid += (a.d.sequences * (K - 1) * (a.d.C / V) + 255) / 256;
+  if (a.dinitial) grid += (a.d.sequences * (K - 1) * (a.d.C / V) + kGradThreads - 1) / kGradThreads;
   if (grid >= INT32_MAX) return cudaErrorInvalidValue;
   *launches = 1;
-  launch_streaming(causal_grad_kernel<T, V, K>, static_cast<unsigned>(grid), 256, 0, s, a, g);
+  launch_streaming(causal_grad_kernel<T, V, K>, static_cast<unsigned>(grid), kGradThreads, 0, s, a, g);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || !a.partial) return e;
   launch_chained(causal_params_kernel<T>, dim3((a.d.C + 31) / 32, K + 1), 512, 0, s, a, static_cast<int>(g.run_blocks / g.channel_blocks));

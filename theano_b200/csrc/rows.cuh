@@ -161,13 +161,17 @@ __device__ __forceinline__ long long start_of(const int* starts, int i, long lon
   const long long s = starts[i];
   return s < 0 ? 0 : s > rows ? rows : s;
 }
-// The last sequence that starts at or before `row`; -1 before the first.
+// The last sequence that starts at or before `row`; -1 before the first.  All lanes of the warp ask for the same row: 32 offsets at a
+// time, one trip to memory for up to 32 sequences, two for 1024.
 __device__ __forceinline__ int sequence_of(const int* starts, int count, long long row, long long rows) {
-  int lo = 0, hi = count;                        // sequences [lo, hi) are undecided
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (start_of(starts, mid, rows) <= row) lo = mid + 1;
-    else hi = mid;
+  int lo = 0, n = count;                         // the sequences before lo start at or before the row, [lo, lo + n) are undecided
+  while (n > 0) {
+    const int step = (n + 31) >> 5, i = (threadIdx.x & 31) * step;
+    const int m = __popc(__ballot_sync(~0u, i < n && start_of(starts, lo + (i < n ? i : 0), rows) <= row));
+    if (m == 0) break;
+    const int end = m * step < n ? m * step : n;
+    n = end - (m - 1) * step - 1;
+    lo += (m - 1) * step + 1;
   }
   return lo - 1;
 }

@@ -176,42 +176,80 @@ __global__ void __launch_bounds__(kScanThreads, S * P <= 32 ? kScanBlocks : 1) s
   }
 }
 
-// One token of every sequence; the states are read, moved on and written where they lie.
-template <typename T, int V, int P>
-__global__ void __launch_bounds__(kScanThreads) scan_step_kernel(ScanArgs a) {
+// One token of every sequence; the states are read, moved on and written where they lie, which is all that takes time.  P lanes share a
+// channel, four states each; QUADS: N is a multiple of four and all rows of states lie on their boundaries, so that they move in 16 bytes.
+// A thread takes kChannels channels a block's width apart, their loads in flight together.
+constexpr int kStepThreads = 128;
+template <typename T, int P, bool QUADS, int kChannels>
+__global__ void __launch_bounds__(kStepThreads) scan_step_kernel(ScanArgs a) {
+  constexpr int kWide = kStepThreads / P;
   pdl_enter();
-  const long long i = blockIdx.x * static_cast<long long>(kScanThreads / P) + threadIdx.x / P;
-  const bool mine = i < a.d.sequences * a.d.C;
-  const int q = threadIdx.x % P, N = a.d.N;
-  const long long seq = mine ? i / a.d.C : 0;
-  const int c = mine ? static_cast<int>(i - seq * a.d.C) : 0, group = c / (a.d.C / a.d.groups);
-  float d = 0.f, x = 0.f, y = 0.f;
-  if (mine) {
-    d = to_float(static_cast<const T*>(a.dt)[seq * a.d.dt.seq + c]) + (a.dt_bias ? a.dt_bias[c] : 0.f);
-    if (a.d.softplus) d = softplus(d);
-    x = to_float(static_cast<const T*>(a.x)[seq * a.d.x.seq + c]);
-    float* state = a.final + (seq * a.d.C + c) * N;
-    const T* B = static_cast<const T*>(a.B) + seq * a.d.B.seq + 1LL * group * N;
-    const T* C = static_cast<const T*>(a.C) + seq * a.d.Cm.seq + 1LL * group * N;
+  const int q = threadIdx.x % P, N = a.d.N, C = a.d.C;
+  const unsigned seq = blockIdx.y;
+  float h[kChannels][4], A[kChannels][4], d[kChannels], x[kChannels], z[kChannels];
+  Pack<T, 4> b[kChannels], w[kChannels];
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int n = 4 * q + s;
-      if (n < N) {
-        const float h = exp2_fast(d * scaled_decay(a.A[1LL * c * N + n])) * state[n] + d * x * to_float(B[n]);
-        state[n] = h;
-        y += h * to_float(C[n]);
-      }
+  for (int k = 0; k < kChannels; ++k) {
+    const int c = (blockIdx.x * kChannels + k) * kWide + threadIdx.x / P, group = c / (C / a.d.groups);
+    d[k] = x[k] = z[k] = 0.f;
+    b[k].clear();
+    w[k].clear();
+#pragma unroll
+    for (int s = 0; s < 4; ++s) h[k][s] = A[k][s] = 0.f;
+    if (c >= C || 4 * q >= N) continue;
+    const float* state = a.final + (1LL * seq * C + c) * N + 4 * q;
+    const float* decay = a.A + 1LL * c * N + 4 * q;
+    const T* B = static_cast<const T*>(a.B) + seq * a.d.B.seq + 1LL * group * N + 4 * q;
+    const T* Cm = static_cast<const T*>(a.C) + seq * a.d.Cm.seq + 1LL * group * N + 4 * q;
+    if (QUADS) {
+      const float4 v = *reinterpret_cast<const float4*>(state), u = *reinterpret_cast<const float4*>(decay);
+      h[k][0] = v.x; h[k][1] = v.y; h[k][2] = v.z; h[k][3] = v.w;
+      A[k][0] = u.x; A[k][1] = u.y; A[k][2] = u.z; A[k][3] = u.w;
+      b[k].load(B);
+      w[k].load(Cm);
+    } else {
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        if (4 * q + s < N) {
+          h[k][s] = state[s];
+          A[k][s] = decay[s];
+          b[k].e[s] = B[s];
+          w[k].e[s] = Cm[s];
+        }
     }
+    d[k] = to_float(static_cast<const T*>(a.dt)[seq * a.d.dt.seq + c]) + (a.dt_bias ? a.dt_bias[c] : 0.f);
+    x[k] = to_float(static_cast<const T*>(a.x)[seq * a.d.x.seq + c]);
+    if (a.z && q == 0) z[k] = to_float(static_cast<const T*>(a.z)[seq * a.d.z.seq + c]);
   }
 #pragma unroll
-  for (int o = 1; o < P; o <<= 1) y += __shfl_xor_sync(~0u, y, o);
-  if (!mine || q) return;
-  if (a.D) y += a.D[c] * x;
-  if (a.z) {
-    const float z = to_float(static_cast<const T*>(a.z)[seq * a.d.z.seq + c]);
-    y *= z * sigmoid(z);
+  for (int k = 0; k < kChannels; ++k) {
+    const int c = (blockIdx.x * kChannels + k) * kWide + threadIdx.x / P;
+    const bool mine = c < C;
+    if (a.d.softplus) d[k] = softplus(d[k]);
+    const float u = d[k] * x[k];
+    float y = 0.f;
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      if (QUADS || 4 * q + s < N) {
+        h[k][s] = exp2_fast(d[k] * scaled_decay(A[k][s])) * h[k][s] + u * b[k].get(s);
+        y += h[k][s] * w[k].get(s);
+      }
+#pragma unroll
+    for (int o = 1; o < P; o <<= 1) y += __shfl_xor_sync(~0u, y, o);
+    if (!mine || 4 * q >= N) continue;
+    float* state = a.final + (1LL * seq * C + c) * N + 4 * q;
+    if (QUADS) {
+      *reinterpret_cast<float4*>(state) = make_float4(h[k][0], h[k][1], h[k][2], h[k][3]);
+    } else {
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+        if (4 * q + s < N) state[s] = h[k][s];
+    }
+    if (q) continue;
+    if (a.D) y = fmaf(a.D[c], x[k], y);
+    if (a.z) y *= z[k] * sigmoid(z[k]);
+    static_cast<T*>(a.y)[seq * a.d.y.seq + c] = from_float<T>(y);
   }
-  static_cast<T*>(a.y)[seq * a.d.y.seq + c] = from_float<T>(y);
 }
 
 }  // namespace
@@ -247,13 +285,41 @@ cudaError_t launch_selective_scan(const ScanArgs& a, int* launches, cudaStream_t
   return a.d.dtype == B200CONV_F16 ? run_type<__half>(a, launches, s) : run_type<__nv_bfloat16>(a, launches, s);
 }
 
+template <typename T, int P, bool QUADS>
+cudaError_t run_step(const ScanArgs& a, cudaStream_t s) {
+  const int wide = kStepThreads / P;
+  // several channels per thread once there are states for every SM's threads
+  const bool many = 1LL * a.d.sequences * a.d.C * P >= 148LL * 2048 * 2;
+  const unsigned blocks = static_cast<unsigned>((a.d.C + (many ? 4 : 1) * wide - 1) / ((many ? 4 : 1) * wide));
+  for (int64_t first = 0; first < a.d.sequences; first += 65535) {
+    ScanArgs b = a;
+    const unsigned n = static_cast<unsigned>(a.d.sequences - first < 65535 ? a.d.sequences - first : 65535);
+    auto on = [&](const void* p, long long stride) { return p ? static_cast<const T*>(p) + first * stride : nullptr; };
+    b.x = on(a.x, a.d.x.seq); b.dt = on(a.dt, a.d.dt.seq); b.z = on(a.z, a.d.z.seq); b.B = on(a.B, a.d.B.seq); b.C = on(a.C, a.d.Cm.seq);
+    b.y = const_cast<T*>(on(a.y, a.d.y.seq));
+    b.final = a.final + first * a.d.C * a.d.N;
+    if (many) launch_streaming(scan_step_kernel<T, P, QUADS, 4>, dim3(blocks, n), kStepThreads, 0, s, b);
+    else launch_streaming(scan_step_kernel<T, P, QUADS, 1>, dim3(blocks, n), kStepThreads, 0, s, b);
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+template <typename T>
+cudaError_t run_step_type(const ScanArgs& a, cudaStream_t s) {
+  const int N = a.d.N;
+  const size_t quad = 4 * sizeof(T);
+  auto whole = [&](const void* p, const b200conv_rows& r) { return reinterpret_cast<uintptr_t>(p) % quad == 0 && r.seq * sizeof(T) % quad == 0; };
+  const bool quads = N % 4 == 0 && aligned16({a.final, a.A}) && whole(a.B, a.d.B) && whole(a.C, a.d.Cm);
+#define B200_LANES(P) if (N <= 4 * P) return quads ? run_step<T, P, true>(a, s) : run_step<T, P, false>(a, s);
+  B200_LANES(2) B200_LANES(4) B200_LANES(8) B200_LANES(16) B200_LANES(32)
+#undef B200_LANES
+  return cudaErrorInvalidValue;
+}
+
 cudaError_t launch_scan_step(const ScanArgs& a, cudaStream_t s) {
-  const long long per = kScanThreads / scan_lanes(a.d.N), grid = (a.d.sequences * a.d.C + per - 1) / per;
-  if (grid >= INT32_MAX) return cudaErrorInvalidValue;
-  return with_scan(a, false, [&](auto t, auto v, auto p) {
-    launch_streaming(scan_step_kernel<decltype(t), 1, decltype(p)::value>, static_cast<unsigned>(grid), kScanThreads, 0, s, a);
-    return cudaGetLastError();
-  });
+  if (a.d.dtype == B200CONV_F32) return run_step_type<float>(a, s);
+  return a.d.dtype == B200CONV_F16 ? run_step_type<__half>(a, s) : run_step_type<__nv_bfloat16>(a, s);
 }
 
 int scan_state_slots(int N) { return N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128; }

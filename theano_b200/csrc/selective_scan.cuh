@@ -82,11 +82,14 @@ __device__ __forceinline__ Piece piece_of(const ScanArgs& a, int id) {
   // Windows of `piece` rows cut the packed tensor; sequence i meets window k in piece i + k: the number grows by one from
   // a window to the next and from a sequence to the next, so that no two pieces share it (and some stay empty).
   const int n = static_cast<int>(a.d.sequences);
-  int lo = 0, hi = n;
-  while (lo < hi) {              // the last sequence whose first piece is not behind `id`
-    const int mid = (lo + hi) >> 1;
-    if (start_of(a.starts, mid, a.d.length) / a.piece + mid <= id) lo = mid + 1;
-    else hi = mid;
+  int lo = 0, left = n;
+  while (left > 0) {             // the last sequence whose first piece is not behind `id`, 32 at a time as in sequence_of
+    const int step = (left + 31) >> 5, i = (threadIdx.x & 31) * step, j = lo + (i < left ? i : 0);
+    const int m = __popc(__ballot_sync(~0u, i < left && start_of(a.starts, j, a.d.length) / a.piece + j <= id));
+    if (m == 0) break;
+    const int end = m * step < left ? m * step : left;
+    left = end - (m - 1) * step - 1;
+    lo += (m - 1) * step + 1;
   }
   p.seq = lo - 1;
   p.base = 0;
@@ -126,22 +129,6 @@ __device__ __forceinline__ void clear_piece_sums(const ScanArgs& a, int id, cons
     a.partial_d[2LL * id * a.d.C + ct.channel + i] = a.partial_d[(2LL * id + 1) * a.d.C + ct.channel + i] = 0.f;
 }
 
-// Four values per lane, summed over P lanes: lane q of each four holds the sum of value q (P >= 4), every lane
-// with P = 1, 2 returns what it is to store below.
-template <int P> __device__ __forceinline__ float lane_sums(const float (&v)[4]) {
-  const int lane = threadIdx.x & 3;
-  // halves change places: after this a lane keeps two of the four sums, over two lanes
-  const bool hi = lane & 2;
-  float a = hi ? v[2] : v[0], b = hi ? v[3] : v[1];
-  a += __shfl_xor_sync(~0u, hi ? v[0] : v[2], 2);
-  b += __shfl_xor_sync(~0u, hi ? v[1] : v[3], 2);
-  const bool odd = lane & 1;
-  float r = (odd ? b : a) + __shfl_xor_sync(~0u, odd ? a : b, 1);
-#pragma unroll
-  for (int o = 4; o < P; o <<= 1) r += __shfl_xor_sync(~0u, r, o);
-  return r;
-}
-
 constexpr int kPolyPairs = 1;                    // pairs of decays that a lane takes by polynomial: none 227, one 210, two 216 us (8192 tokens, 2048 channels)
 constexpr int tile_tokens(int NS) { return NS <= 32 ? 32 : 1024 / NS; }           // of a tile of B and C
 
@@ -169,27 +156,5 @@ struct StateRows {
     }
   }
 };
-
-// f(type, pieces of V elements, lanes per channel) for the call's data type and state size
-template <typename T, int V, class F> cudaError_t with_lanes(int N, F f) {
-#define B200_LANES(P) if (N <= 4 * P) return f(T(), std::integral_constant<int, (V < kScanThreads / P ? V : kScanThreads / P)>(), std::integral_constant<int, P>());
-  B200_LANES(4) B200_LANES(8) B200_LANES(16) B200_LANES(32)
-#undef B200_LANES
-  return cudaErrorInvalidValue;
-}
-template <class F> cudaError_t with_scan(const ScanArgs& a, bool wide, F f) {
-  if (a.d.dtype == B200CONV_F32) return wide ? with_lanes<float, 4>(a.d.N, f) : with_lanes<float, 1>(a.d.N, f);
-  if (a.d.dtype == B200CONV_F16) return wide ? with_lanes<__half, 8>(a.d.N, f) : with_lanes<__half, 1>(a.d.N, f);
-  return wide ? with_lanes<__nv_bfloat16, 8>(a.d.N, f) : with_lanes<__nv_bfloat16, 1>(a.d.N, f);
-}
-inline int scan_lanes(int N) { return N <= 16 ? 4 : N <= 32 ? 8 : N <= 64 ? 16 : 32; }
-
-// Whether pieces of 16 bytes lie on their boundaries in the tensors of channels, and none straddles two groups.
-inline bool wide_scan(const ScanArgs& a) {
-  const int dt = a.d.dtype, V = dt == B200CONV_F32 ? 4 : 8;
-  return a.d.C / a.d.groups % V == 0 && rows_aligned(a.x, a.d.x, dt) && rows_aligned(a.dt, a.d.dt, dt) && rows_aligned(a.z, a.d.z, dt) &&
-         rows_aligned(a.y, a.d.y, dt) && rows_aligned(a.dy, a.d.dy, dt) && rows_aligned(a.dx, a.d.dx, dt) && rows_aligned(a.ddt, a.d.ddt, dt) &&
-         rows_aligned(a.dz, a.d.dz, dt);
-}
 
 }  // namespace b200
