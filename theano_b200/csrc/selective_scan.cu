@@ -176,80 +176,84 @@ __global__ void __launch_bounds__(kScanThreads, S * P <= 32 ? kScanBlocks : 1) s
   }
 }
 
-// One token of every sequence; the states are read, moved on and written where they lie, which is all that takes time.  P lanes share a
-// channel, four states each; QUADS: N is a multiple of four and all rows of states lie on their boundaries, so that they move in 16 bytes.
-// A thread takes kChannels channels a block's width apart, their loads in flight together.
+// One token of every sequence; the states are read, moved on and written where they lie, which is all that takes time once the work per
+// channel is out of the way: P lanes share a channel, eight states each (four each: 27 us for 256 sequences of 2048 channels and 16
+// states, eight 20).  QUADS: N is a multiple of four and all rows of states lie on their boundaries, so that they move in 16 bytes.
 constexpr int kStepThreads = 128;
-template <typename T, int P, bool QUADS, int kChannels>
+template <typename T, int P, bool QUADS>
 __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(ScanArgs a) {
   constexpr int kWide = kStepThreads / P;
   pdl_enter();
-  const int q = threadIdx.x % P, N = a.d.N, C = a.d.C;
+  const int q = threadIdx.x % P, N = a.d.N, C = a.d.C, n0 = 8 * q;
   const unsigned seq = blockIdx.y;
-  float h[kChannels][4], A[kChannels][4], d[kChannels], x[kChannels], z[kChannels];
-  Pack<T, 4> b[kChannels], w[kChannels];
+  const int c = blockIdx.x * kWide + threadIdx.x / P;
+  const bool mine = c < C;
+  const int group = a.d.groups == 1 || !mine ? 0 : c / (C / a.d.groups);
+  float h[8], A[8];
+  Pack<T, 4> b[2], w[2];
+  float d = 0.f, x = 0.f, z = 0.f;
+  float* state = a.final + (1LL * seq * C + c) * N + n0;
 #pragma unroll
-  for (int k = 0; k < kChannels; ++k) {
-    const int c = (blockIdx.x * kChannels + k) * kWide + threadIdx.x / P, group = c / (C / a.d.groups);
-    d[k] = x[k] = z[k] = 0.f;
-    b[k].clear();
-    w[k].clear();
+  for (int j = 0; j < 2; ++j) {
+    b[j].clear();
+    w[j].clear();
 #pragma unroll
-    for (int s = 0; s < 4; ++s) h[k][s] = A[k][s] = 0.f;
-    if (c >= C || 4 * q >= N) continue;
-    const float* state = a.final + (1LL * seq * C + c) * N + 4 * q;
-    const float* decay = a.A + 1LL * c * N + 4 * q;
-    const T* B = static_cast<const T*>(a.B) + seq * a.d.B.seq + 1LL * group * N + 4 * q;
-    const T* Cm = static_cast<const T*>(a.C) + seq * a.d.Cm.seq + 1LL * group * N + 4 * q;
-    if (QUADS) {
-      const float4 v = *reinterpret_cast<const float4*>(state), u = *reinterpret_cast<const float4*>(decay);
-      h[k][0] = v.x; h[k][1] = v.y; h[k][2] = v.z; h[k][3] = v.w;
-      A[k][0] = u.x; A[k][1] = u.y; A[k][2] = u.z; A[k][3] = u.w;
-      b[k].load(B);
-      w[k].load(Cm);
-    } else {
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-        if (4 * q + s < N) {
-          h[k][s] = state[s];
-          A[k][s] = decay[s];
-          b[k].e[s] = B[s];
-          w[k].e[s] = Cm[s];
-        }
-    }
-    d[k] = to_float(static_cast<const T*>(a.dt)[seq * a.d.dt.seq + c]) + (a.dt_bias ? a.dt_bias[c] : 0.f);
-    x[k] = to_float(static_cast<const T*>(a.x)[seq * a.d.x.seq + c]);
-    if (a.z && q == 0) z[k] = to_float(static_cast<const T*>(a.z)[seq * a.d.z.seq + c]);
+    for (int s = 0; s < 4; ++s) h[4 * j + s] = A[4 * j + s] = 0.f;
   }
+  if (mine) {
+    const float* decay = a.A + 1LL * c * N + n0;
+    const T* B = static_cast<const T*>(a.B) + seq * a.d.B.seq + 1LL * group * N + n0;
+    const T* Cm = static_cast<const T*>(a.C) + seq * a.d.Cm.seq + 1LL * group * N + n0;
 #pragma unroll
-  for (int k = 0; k < kChannels; ++k) {
-    const int c = (blockIdx.x * kChannels + k) * kWide + threadIdx.x / P;
-    const bool mine = c < C;
-    if (a.d.softplus) d[k] = softplus(d[k]);
-    const float u = d[k] * x[k];
-    float y = 0.f;
+    for (int j = 0; j < 2; ++j) {
+      if (n0 + 4 * j >= N) continue;
+      if (QUADS) {
+        const float4 v = reinterpret_cast<const float4*>(state)[j], u = reinterpret_cast<const float4*>(decay)[j];
+        h[4 * j] = v.x; h[4 * j + 1] = v.y; h[4 * j + 2] = v.z; h[4 * j + 3] = v.w;
+        A[4 * j] = u.x; A[4 * j + 1] = u.y; A[4 * j + 2] = u.z; A[4 * j + 3] = u.w;
+        b[j].load(B + 4 * j);
+        w[j].load(Cm + 4 * j);
+      } else {
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
-      if (QUADS || 4 * q + s < N) {
-        h[k][s] = exp2_fast(d[k] * scaled_decay(A[k][s])) * h[k][s] + u * b[k].get(s);
-        y += h[k][s] * w[k].get(s);
+        for (int s = 0; s < 4; ++s)
+          if (n0 + 4 * j + s < N) {
+            h[4 * j + s] = state[4 * j + s];
+            A[4 * j + s] = decay[4 * j + s];
+            b[j].e[s] = B[4 * j + s];
+            w[j].e[s] = Cm[4 * j + s];
+          }
       }
+    }
+    d = to_float(static_cast<const T*>(a.dt)[seq * a.d.dt.seq + c]) + (a.dt_bias ? a.dt_bias[c] : 0.f);
+    x = to_float(static_cast<const T*>(a.x)[seq * a.d.x.seq + c]);
+    if (a.z) z = to_float(static_cast<const T*>(a.z)[seq * a.d.z.seq + c]);
+  }
+  if (a.d.softplus) d = softplus(d);
+  const float u = d * x;
+  float y = 0.f;
 #pragma unroll
-    for (int o = 1; o < P; o <<= 1) y += __shfl_xor_sync(~0u, y, o);
-    if (!mine || 4 * q >= N) continue;
-    float* state = a.final + (1LL * seq * C + c) * N + 4 * q;
+  for (int i = 0; i < 8; ++i) {
+    h[i] = exp2_fast(d * scaled_decay(A[i])) * h[i] + u * b[i / 4].get(i % 4);
+    if (n0 + i < N) y += h[i] * w[i / 4].get(i % 4);
+  }
+#pragma unroll
+  for (int o = 1; o < P; o <<= 1) y += __shfl_xor_sync(~0u, y, o);
+  if (!mine) return;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    if (n0 + 4 * j >= N) break;
     if (QUADS) {
-      *reinterpret_cast<float4*>(state) = make_float4(h[k][0], h[k][1], h[k][2], h[k][3]);
+      reinterpret_cast<float4*>(state)[j] = make_float4(h[4 * j], h[4 * j + 1], h[4 * j + 2], h[4 * j + 3]);
     } else {
 #pragma unroll
       for (int s = 0; s < 4; ++s)
-        if (4 * q + s < N) state[s] = h[k][s];
+        if (n0 + 4 * j + s < N) state[4 * j + s] = h[4 * j + s];
     }
-    if (q) continue;
-    if (a.D) y = fmaf(a.D[c], x[k], y);
-    if (a.z) y *= z[k] * sigmoid(z[k]);
-    static_cast<T*>(a.y)[seq * a.d.y.seq + c] = from_float<T>(y);
   }
+  if (q) return;
+  if (a.D) y = fmaf(a.D[c], x, y);
+  if (a.z) y *= z * sigmoid(z);
+  static_cast<T*>(a.y)[seq * a.d.y.seq + c] = from_float<T>(y);
 }
 
 }  // namespace
@@ -288,9 +292,7 @@ cudaError_t launch_selective_scan(const ScanArgs& a, int* launches, cudaStream_t
 template <typename T, int P, bool QUADS>
 cudaError_t run_step(const ScanArgs& a, cudaStream_t s) {
   const int wide = kStepThreads / P;
-  // several channels per thread once there are states for every SM's threads
-  const bool many = 1LL * a.d.sequences * a.d.C * P >= 148LL * 2048 * 2;
-  const unsigned blocks = static_cast<unsigned>((a.d.C + (many ? 4 : 1) * wide - 1) / ((many ? 4 : 1) * wide));
+  const unsigned blocks = static_cast<unsigned>((a.d.C + wide - 1) / wide);
   for (int64_t first = 0; first < a.d.sequences; first += 65535) {
     ScanArgs b = a;
     const unsigned n = static_cast<unsigned>(a.d.sequences - first < 65535 ? a.d.sequences - first : 65535);
@@ -298,8 +300,7 @@ cudaError_t run_step(const ScanArgs& a, cudaStream_t s) {
     b.x = on(a.x, a.d.x.seq); b.dt = on(a.dt, a.d.dt.seq); b.z = on(a.z, a.d.z.seq); b.B = on(a.B, a.d.B.seq); b.C = on(a.C, a.d.Cm.seq);
     b.y = const_cast<T*>(on(a.y, a.d.y.seq));
     b.final = a.final + first * a.d.C * a.d.N;
-    if (many) launch_streaming(scan_step_kernel<T, P, QUADS, 4>, dim3(blocks, n), kStepThreads, 0, s, b);
-    else launch_streaming(scan_step_kernel<T, P, QUADS, 1>, dim3(blocks, n), kStepThreads, 0, s, b);
+    launch_streaming(scan_step_kernel<T, P, QUADS>, dim3(blocks, n), kStepThreads, 0, s, b);
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
@@ -311,8 +312,8 @@ cudaError_t run_step_type(const ScanArgs& a, cudaStream_t s) {
   const size_t quad = 4 * sizeof(T);
   auto whole = [&](const void* p, const b200conv_rows& r) { return reinterpret_cast<uintptr_t>(p) % quad == 0 && r.seq * sizeof(T) % quad == 0; };
   const bool quads = N % 4 == 0 && aligned16({a.final, a.A}) && whole(a.B, a.d.B) && whole(a.C, a.d.Cm);
-#define B200_LANES(P) if (N <= 4 * P) return quads ? run_step<T, P, true>(a, s) : run_step<T, P, false>(a, s);
-  B200_LANES(2) B200_LANES(4) B200_LANES(8) B200_LANES(16) B200_LANES(32)
+#define B200_LANES(P) if (N <= 8 * P) return quads ? run_step<T, P, true>(a, s) : run_step<T, P, false>(a, s);
+  B200_LANES(1) B200_LANES(2) B200_LANES(4) B200_LANES(8) B200_LANES(16)
 #undef B200_LANES
   return cudaErrorInvalidValue;
 }

@@ -4,8 +4,6 @@
 // warp holds 32 / P channels.  Sequences may be cut into pieces of `piece` tokens that blocks take independently; what a piece
 // does to a state is h -> exp(A sum of delta) h + (its own result from zero), so pieces are joined by one exponential each.
 #pragma once
-#include <math_constants.h>
-
 #include <type_traits>
 
 #include "internal.h"
@@ -54,8 +52,9 @@ __device__ __forceinline__ Pair exp2_pair(Pair a) {
 // A log2(e).  A decay of minus infinity ends a state in any step of positive size and, like every other, not in one of size zero
 // (as which the tokens behind a piece count).
 __device__ __forceinline__ float scaled_decay(float A) {
-  const float v = A * kLog2e;
-  return v == -CUDART_INF_F ? -3.4e38f : v;
+  float v;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(A * kLog2e), "f"(-3.4e38f));
+  return v;
 }
 
 // The tokens of a piece: sequence `seq`, its tokens [from, to) counted from the tensor's row `row0` of that sequence.

@@ -10,6 +10,7 @@ The reference runs causal convolutions through its 2-D convolution (theano/tenso
 recurrences through its scan op, one op call per token; nothing here computes on the CPU.
 """
 import ctypes
+import itertools
 
 import numpy as np
 
@@ -23,6 +24,21 @@ _CODES = {np.dtype(np.float32): F32, np.dtype(np.float16): F16, BFLOAT16: BF16}
 _DTYPES = {F32: np.dtype(np.float32), F16: np.dtype(np.float16), BF16: BFLOAT16}
 _INT32 = np.dtype(np.int32)
 _OTHER = -1                              # code of tensors that are no operands (offsets)
+
+
+_signatures = {}                         # what plans need to know of an array -> a number that stands for it
+_numbers = itertools.count(1)
+
+
+def _signature(*what):
+    """A number for a shape with its strides and type: plans are looked up on every call, and hashing ten nested tuples cost
+    as much host time as the launch.  Equal signatures may get two numbers (the table is emptied at times), never two one."""
+    n = _signatures.get(what)
+    if n is None:
+        if len(_signatures) >= 1 << 16:
+            _signatures.clear()
+        n = _signatures[what] = next(_numbers)
+    return n
 
 
 def _dtype(dt):
@@ -66,7 +82,7 @@ class DeviceArray(object):
             raise ValueError("the last axis must be contiguous and no stride negative: shape %s, strides %s" % (self.shape, self.strides))
         self.stored, self._base = int(stored), _base
         self.code = _CODES.get(self.dtype, _OTHER)
-        self.sig = (self.shape, self.strides, self.code, self.stored)
+        self.sig = _signature(self.shape, self.strides, self.code, self.stored)
         self.owner = _ptr is None
         self.ptr = ctx.malloc(self.size * self.dtype.itemsize) if self.owner else _ptr
 
@@ -164,7 +180,7 @@ class Sequences(object):
         self.lengths = tuple(int(n) for n in lengths)
         self.total, self.longest = int(lengths.astype(np.int64).sum()), int(lengths.max())
         self.starts = DeviceArray.from_host(ctx, np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32))
-        self.sig = (self.count, self.total, self.longest)
+        self.sig = _signature("sequences", self.count, self.total, self.longest)
 
 
 # ======================================================================================
@@ -211,7 +227,7 @@ def _array(t):
 
 
 def _sig(t):
-    return None if t is None else t.sig
+    return 0 if t is None else t.sig
 
 
 def _ptr(t):
