@@ -649,3 +649,94 @@ def device_selective_scan_grad(dy, x, dt, A, B, C, D=None, z=None, dt_bias=None,
     if rc:
         ctx.check(rc)
     return grads
+
+
+# ======================================================================================
+# numpy in / numpy out (float32 and float16; synchronous)
+# ======================================================================================
+def _upload(ctx, dtype, *arrays):
+    return [None if a is None else DeviceArray.from_host(ctx, np.asarray(a), dtype) for a in arrays]
+
+
+def _common_dtype(*arrays):
+    dt = np.result_type(*[np.asarray(a).dtype for a in arrays if a is not None])
+    if dt not in (np.dtype(np.float32), np.dtype(np.float16)):
+        raise TypeError("sequence operators on host arrays handle float32 and float16, not %s" % dt)
+    return dt
+
+
+def layer_norm(x, gamma=None, beta=None, eps=1e-5, ctx=None):
+    """Layer norm over the last axis of a host array of (rows, channels) or (sequences, tokens, channels)."""
+    dt = _common_dtype(x, gamma, beta)
+    ctx = ctx or shim.get_context()
+    x, gamma, beta = _upload(ctx, dt, x, gamma, beta)
+    return device_layer_norm(x, gamma, beta, eps).to_host()
+
+
+def layer_norm_grad(dy, x, gamma=None, eps=1e-5, ctx=None):
+    """Gradients (dx, dgamma, dbeta) of `layer_norm`; without gamma those of gamma and beta are float32."""
+    dt = _common_dtype(dy, x, gamma)
+    ctx = ctx or shim.get_context()
+    dy, x, gamma = _upload(ctx, dt, dy, x, gamma)
+    stats = DeviceArray(ctx, x.shape[:-1] + (2,), np.float32)
+    device_layer_norm(x, gamma, None, eps, stats=stats)
+    return tuple(t.to_host() for t in device_layer_norm_grad(dy, x, gamma, stats))
+
+
+def causal_conv1d(x, w, bias=None, silu=False, filter_flip=True, initial=None, lengths=None, ctx=None):
+    """`device_causal_conv1d` on host arrays; returns (y, final state).  `lengths`: of packed sequences."""
+    dt = _common_dtype(x, w, bias, initial)
+    ctx = ctx or shim.get_context()
+    x, w, bias, initial = _upload(ctx, dt, x, w, bias, initial)
+    seqs = None if lengths is None else Sequences(ctx, lengths)
+    S, _, C = _batch(x, seqs, "a causal convolution")
+    final = DeviceArray(ctx, (S, max(w.shape[-1] - 1, 0), C), dt)
+    y = device_causal_conv1d(x, w, bias, silu, filter_flip, initial=initial, final=final, sequences=seqs, out=_zeros(ctx, x.shape, dt))
+    return y.to_host(), final.to_host()
+
+
+def causal_conv1d_grad(dy, x, w, bias=None, silu=False, filter_flip=True, initial=None, lengths=None, ctx=None):
+    """Gradients (dx, dw, dbias, dinitial) of `causal_conv1d`; None for those of absent inputs, zeros in rows of no sequence."""
+    dt = _common_dtype(dy, x, w, bias, initial)
+    ctx = ctx or shim.get_context()
+    dy, x, w, bias, initial = _upload(ctx, dt, dy, x, w, bias, initial)
+    seqs = None if lengths is None else Sequences(ctx, lengths)
+    grads = device_causal_conv1d_grad(dy, x, w, bias, silu, filter_flip, initial=initial, sequences=seqs, out=_zeros(ctx, x.shape, dt),
+                                      dinitial=None if initial is None else DeviceArray(ctx, initial.shape, dt))
+    return tuple(None if t is None else t.to_host() for t in grads)
+
+
+def _scan_inputs(ctx, dt, x, dts, A, B, C, D, z, dt_bias, initial, lengths):
+    x, dts, B, C, z = _upload(ctx, dt, x, dts, B, C, z)
+    A, D, dt_bias, initial = _upload(ctx, np.float32, A, D, dt_bias, initial)
+    return (x, dts, A, B, C), dict(D=D, z=z, dt_bias=dt_bias, initial=initial, sequences=None if lengths is None else Sequences(ctx, lengths))
+
+
+def _zeros(ctx, shape, dt):
+    t = DeviceArray(ctx, shape, dt)
+    ctx.memset(t.ptr, 0, t.size * t.dtype.itemsize)
+    return t
+
+
+def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=False, initial=None, lengths=None, ctx=None):
+    """`device_selective_scan` on host arrays; returns (y, final states).  `lengths`: of packed sequences."""
+    dtype = _common_dtype(x, dt, B, C, z)
+    ctx = ctx or shim.get_context()
+    args, more = _scan_inputs(ctx, dtype, x, dt, A, B, C, D, z, dt_bias, initial, lengths)
+    S = more["sequences"].count if lengths is not None else args[0].shape[0]
+    final = DeviceArray(ctx, (S,) + args[2].shape, np.float32)
+    y = device_selective_scan(*args, softplus=softplus, final=final, out=_zeros(ctx, args[0].shape, dtype), **more)
+    return y.to_host(), final.to_host()
+
+
+def selective_scan_grad(dy, x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=False, initial=None, dfinal=None, lengths=None, ctx=None):
+    """Gradients of `selective_scan` by input name (`device_selective_scan_grad`); zeros in rows of no sequence."""
+    dtype = _common_dtype(dy, x, dt, B, C, z)
+    ctx = ctx or shim.get_context()
+    args, more = _scan_inputs(ctx, dtype, x, dt, A, B, C, D, z, dt_bias, initial, lengths)
+    dy, = _upload(ctx, dtype, dy)
+    dfinal, = _upload(ctx, np.float32, dfinal)
+    named = dict(x=args[0], dt=args[1], B=args[3], C=args[4], z=more["z"])
+    grads = {k: _zeros(ctx, t.shape, dtype) for k, t in named.items() if t is not None}
+    grads = device_selective_scan_grad(dy, *args, softplus=softplus, dfinal=dfinal, grads=grads, **more)
+    return {k: t.to_host() for k, t in grads.items()}
