@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kScanThreads, P == 1 ? kGradBlocks : 1) scan_g
       h[s] = CUT && have && a.initial ? a.initial[at] : 0.f;
     }
     if (CUT && mine) {
-#pragma unroll 2
+#pragma unroll 4
       for (int j = p.last; j > id; --j) {
         const long long o = 1LL * j * a.d.C + c;
         const float4* b = reinterpret_cast<const float4*>(a.piece_back + o * NS + q * 16);
@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(kScanThreads, P == 1 ? kGradBlocks : 1) scan_g
           g[4 * s + 3] = v.w + exp2_fast(A_[4 * s + 3] * all) * g[4 * s + 3];
         }
       }
-#pragma unroll 2
+#pragma unroll 4
       for (int j = p.first; j < id; ++j) {
         const long long o = 1LL * j * a.d.C + c;
         const float4* b = reinterpret_cast<const float4*>(a.piece_state + o * NS + q * 16);
@@ -315,11 +315,21 @@ __global__ void __launch_bounds__(kScanThreads, P == 1 ? kGradBlocks : 1) scan_g
           const int t = i / (kWide / kVec), cc = i % (kWide / kVec) * kVec;
           if (t < n && cc < ct.channels) copy_async(&sh.rows[turn][w][t][cc], src + (tok + t) * row + cc);
         }
-      } else {
-        for (int i = threadIdx.x; i < kStep * kWide; i += kScanThreads) {
-          const int t = i / kWide, cc = i % kWide;
-          if (t < n && cc < ct.channels) sh.rows[turn][w][t][cc] = src[(tok + t) * row + cc];
+      } else if (sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < kStep * kWide / kScanThreads; ++k) {
+          const int i = threadIdx.x + k * kScanThreads, t = i / kWide, cc = i % kWide;
+          if (t < n && cc < ct.channels) copy_async_4(&sh.rows[turn][w][t][cc], src + (tok + t) * row + cc);
         }
+      } else {
+        T v[kStep * kWide / kScanThreads];       // all on their way before the first is needed
+#pragma unroll
+        for (int k = 0; k < kStep * kWide / kScanThreads; ++k) {
+          const int i = threadIdx.x + k * kScanThreads, t = i / kWide, cc = i % kWide;
+          v[k] = t < n && cc < ct.channels ? src[(tok + t) * row + cc] : from_float<T>(0.f);
+        }
+#pragma unroll
+        for (int k = 0; k < kStep * kWide / kScanThreads; ++k) (&sh.rows[turn][w][0][0])[threadIdx.x + k * kScanThreads] = v[k];
       }
     }
     if (mine) {
