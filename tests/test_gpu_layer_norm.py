@@ -190,3 +190,41 @@ def test_same_bits_every_time_and_in_a_graph():
     other.launch()
     graph.launch()
     assert all(np.array_equal(a, t.to_host()) for a, t in zip(first, [y] + outs))
+
+
+@TYPES
+@pytest.mark.parametrize("C", [24, 300, 20001])
+@pytest.mark.parametrize("over", ["dy", "dtotal"])
+def test_gradient_over_its_input(dt, C, over):
+    """dx in the place of dy or of the gradient that is added: the bits of a call with an array of its own."""
+    ctx, dtype = shim.get_context(0), DTYPES[dt]
+    rs = np.random.RandomState(C)
+    x, dy, extra = (normal(rs, (2, 5, C), dtype) for _ in range(3))
+    X, G, stats = put(ctx, x, dtype), put(ctx, normal(rs, (C,), dtype), dtype), Q.DeviceArray(ctx, (2, 5, 2), np.float32)
+    Q.device_layer_norm(X, G, None, EPS, stats=stats)
+    t = dict(dy=put(ctx, dy, dtype), dtotal=put(ctx, extra, dtype))
+    want = [a.to_host() for a in Q.device_layer_norm_grad(t["dy"], X, G, stats, dtotal=t["dtotal"])]
+    got = [a.to_host() for a in Q.device_layer_norm_grad(t["dy"], X, G, stats, dtotal=t["dtotal"], out=t[over])]
+    assert all(np.array_equal(a, b) for a, b in zip(got, want))
+
+
+def test_elements_off_their_boundaries_are_refused():
+    ctx = shim.get_context(0)
+    a = Q.DeviceArray(ctx, (2, 3, 8), np.float32)
+    for off in (1, 2):
+        bad = Q.DeviceArray(ctx, (1, 3, 8), np.float32, (24, 8, 1), a.ptr + off)
+        with pytest.raises(ValueError):
+            Q.device_layer_norm(bad)
+    half = Q.DeviceArray(ctx, (1, 3, 8), np.float16, (24, 8, 1), a.ptr + 2)
+    Q.device_layer_norm(half, out=Q.DeviceArray(ctx, (1, 3, 8), np.float16))
+    with pytest.raises(ValueError):
+        Q.device_layer_norm(a[:1], stats=Q.DeviceArray(ctx, (1, 3, 2), np.float32, (6, 2, 1), a.ptr + 4))
+    ctx.sync()
+
+
+def test_no_channels_refused_by_the_library():
+    ctx = shim.get_context(0)
+    d = Q.NormDesc(1, 1, 0, Q.F32, 0, 0.0)
+    assert ctx.lib.b200conv_layer_norm(ctx.h, Q.ctypes.byref(d), None, None, None, None, None, None, None) == shim.E_INVALID
+    assert ctx.lib.b200conv_layer_norm(ctx.h, None, None, None, None, None, None, None, None) == shim.E_INVALID
+    assert ctx.lib.b200conv_layer_norm(None, Q.ctypes.byref(d), None, None, None, None, None, None, None) == shim.E_INVALID

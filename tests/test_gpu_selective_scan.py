@@ -188,3 +188,16 @@ def test_same_bits_every_time_and_in_a_graph():
     other.launch()
     graph.launch()
     assert np.array_equal(first[0], y.to_host()) and np.array_equal(first[1], final.to_host())
+
+
+def test_steps_of_more_sequences_than_a_grid_is_high():
+    """65536 and more sequences: the states behind the 65535th move on as the first ones."""
+    ctx = shim.get_context(0)
+    S, C, N = 65540, 2, 4
+    one = lambda *s: put(ctx, np.ones(s), np.float32)  # noqa: E731
+    state = put(ctx, np.tile(np.arange(C * N, dtype=np.float32).reshape(1, C, N), (S, 1, 1)), np.float32)
+    y = Q.device_selective_scan_step(one(S, C), one(S, C), put(ctx, -np.ones((C, N)), np.float32), one(S, N), one(S, N), state).to_host()
+    h = state.to_host()
+    assert (h == h[:1]).all() and (y == y[:1]).all()
+    # one decay of e^-1 and a step of one: 4 roundings of 2^-24 of the value, of which exp2's 2^-22 is the largest
+    assert np.abs(h[0] - (np.arange(8).reshape(C, N) * np.exp(-1) + 1)).max() < 8 * 2 ** -22

@@ -3376,10 +3376,17 @@ int b200conv_channel_sum(b200conv_ctx* c, const void* x, void* out, long long pi
 }
 
 // ---- sequence operators -------------------------------------------------------------------
-// Checks that they share: types, sizes and strides.  Pointers to device memory cannot be looked into.
-static int check_rows(b200conv_ctx* c, const char* name, const void* p, const b200conv_rows& r, long long sequences, long long length, int C,
+// Checks that they share: types, sizes, strides and that elements lie on their own boundaries.
+static int check_aligned(b200conv_ctx* c, std::initializer_list<const void*> ptrs, size_t bytes) {
+  for (const void* p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) % bytes) return fail(c, B200CONV_E_INVALID, "array at %p: elements of %zu bytes off their boundaries", p, bytes);
+  return 0;
+}
+static int check_rows(b200conv_ctx* c, const char* name, const void* p, const b200conv_rows& r, long long sequences, long long length, int C, int dtype,
                       bool written = false) {
   if (!p || sequences * length == 0) return 0;
+  const int rc = check_aligned(c, {p}, row_elem_size(dtype));
+  if (rc) return rc;
   if (r.stored < 0 || r.row < 0 || r.seq < 0) return fail(c, B200CONV_E_INVALID, "%s: negative stride", name);
   const long long stored = std::max(C, r.stored);
   if (written && ((length > 1 && r.row < stored) || (sequences > 1 && r.seq < stored)))
@@ -3391,6 +3398,7 @@ static int check_sizes(b200conv_ctx* c, long long sequences, long long length, l
   if (dtype != B200CONV_F32 && dtype != B200CONV_F16 && dtype != B200CONV_BF16)
     return fail(c, B200CONV_E_INVALID, "dtype must be float32, float16 or bfloat16");
   if (sequences < 0 || length < 0 || C < 0) return fail(c, B200CONV_E_INVALID, "negative dimension");
+  if (C > INT32_MAX / 2) return fail(c, B200CONV_E_UNSUPPORTED, "%lld channels", C);
   if (sequences > INT32_MAX || length > INT32_MAX || sequences * length > INT32_MAX)
     return fail(c, B200CONV_E_UNSUPPORTED, "more than 2^31 - 1 rows (%lld sequences of %lld)", sequences, length);
   return 0;
@@ -3408,9 +3416,10 @@ int b200conv_layer_norm(b200conv_ctx* c, const b200conv_norm_desc* d, const void
   if (!(d->eps >= 0.f)) return fail(c, B200CONV_E_INVALID, "eps must not be negative");
   if (d->sequences * d->length == 0) return 0;
   if (!x || !y) return fail(c, B200CONV_E_INVALID, "layer norm without input or output");
-  if ((rc = check_rows(c, "x", x, d->x, d->sequences, d->length, d->C)) || (rc = check_rows(c, "residual", residual, d->residual, d->sequences, d->length, d->C)) ||
-      (rc = check_rows(c, "y", y, d->y, d->sequences, d->length, d->C, true)) || (rc = check_rows(c, "total", total, d->total, d->sequences, d->length, d->C, true)))
+  if ((rc = check_rows(c, "x", x, d->x, d->sequences, d->length, d->C, d->dtype)) || (rc = check_rows(c, "residual", residual, d->residual, d->sequences, d->length, d->C, d->dtype)) ||
+      (rc = check_rows(c, "y", y, d->y, d->sequences, d->length, d->C, d->dtype, true)) || (rc = check_rows(c, "total", total, d->total, d->sequences, d->length, d->C, d->dtype, true)))
     return rc;
+  if ((rc = check_aligned(c, {gamma, beta}, d->param_f32 ? 4 : row_elem_size(d->dtype))) || (rc = check_aligned(c, {stats}, 8))) return rc;
   NormArgs a = {};
   a.d = *d;
   a.x = x; a.residual = residual; a.gamma = gamma; a.beta = beta; a.y = y; a.total = total; a.stats = stats;
@@ -3434,9 +3443,10 @@ int b200conv_layer_norm_grad(b200conv_ctx* c, const b200conv_norm_desc* d, const
     return 0;
   }
   if (!x || !dy || !stats || !dx) return fail(c, B200CONV_E_INVALID, "layer norm gradient without dy, x, stats or dx");
-  if ((rc = check_rows(c, "x", x, d->x, d->sequences, d->length, d->C)) || (rc = check_rows(c, "dy", dy, d->dy, d->sequences, d->length, d->C)) ||
-      (rc = check_rows(c, "dtotal", dtotal, d->dtotal, d->sequences, d->length, d->C)) || (rc = check_rows(c, "dx", dx, d->dx, d->sequences, d->length, d->C, true)))
+  if ((rc = check_rows(c, "x", x, d->x, d->sequences, d->length, d->C, d->dtype)) || (rc = check_rows(c, "dy", dy, d->dy, d->sequences, d->length, d->C, d->dtype)) ||
+      (rc = check_rows(c, "dtotal", dtotal, d->dtotal, d->sequences, d->length, d->C, d->dtype)) || (rc = check_rows(c, "dx", dx, d->dx, d->sequences, d->length, d->C, d->dtype, true)))
     return rc;
+  if ((rc = check_aligned(c, {gamma, dgamma, dbeta}, d->param_f32 ? 4 : row_elem_size(d->dtype))) || (rc = check_aligned(c, {stats}, 8))) return rc;
   Scratch tmp(c);
   NormArgs a = {};
   a.d = *d;
@@ -3467,7 +3477,8 @@ static int detach_state(b200conv_ctx* c, Scratch& tmp, const void** initial, con
   return 0;
 }
 
-static int check_causal(b200conv_ctx* c, const b200conv_causal_desc* d, const void* x, const void* w, const int32_t* starts) {
+static int check_causal(b200conv_ctx* c, const b200conv_causal_desc* d, const void* x, const void* w, const void* bias, const void* initial, const void* final,
+                        const int32_t* starts) {
   if (!d) return fail(c, B200CONV_E_INVALID, "null descriptor");
   int rc = check_sizes(c, d->packed ? 1 : d->sequences, d->length, d->C, d->dtype);
   if (rc) return rc;
@@ -3477,7 +3488,10 @@ static int check_causal(b200conv_ctx* c, const b200conv_causal_desc* d, const vo
   const bool any = d->sequences && d->length && d->C;
   if (any && !x) return fail(c, B200CONV_E_INVALID, "causal convolution without input");
   if (d->C && !w) return fail(c, B200CONV_E_INVALID, "causal convolution without filters");
-  return check_rows(c, "x", x, d->x, d->packed ? 1 : d->sequences, d->length, d->C);
+  if ((rc = check_aligned(c, {w, bias}, d->param_f32 ? 4 : row_elem_size(d->dtype))) || (rc = check_aligned(c, {initial, final}, row_elem_size(d->dtype))) ||
+      (rc = check_aligned(c, {starts}, 4)))
+    return rc;
+  return check_rows(c, "x", x, d->x, d->packed ? 1 : d->sequences, d->length, d->C, d->dtype);
 }
 static size_t causal_state_bytes(const b200conv_causal_desc* d) {
   return row_elem_size(d->dtype) * static_cast<size_t>(d->sequences) * (d->width - 1) * d->C;
@@ -3488,8 +3502,8 @@ int b200conv_causal_conv(b200conv_ctx* c, const b200conv_causal_desc* d, const v
   if (!c) return B200CONV_E_INVALID;
   std::lock_guard<std::mutex> g(c->mu);
   DeviceGuard dg(c->device);
-  int rc = check_causal(c, d, x, w, starts);
-  if (rc || (rc = check_rows(c, "y", y, d->y, d->packed ? 1 : d->sequences, d->length, d->C, true))) return rc;
+  int rc = check_causal(c, d, x, w, bias, initial, final, starts);
+  if (rc || (rc = check_rows(c, "y", y, d->y, d->packed ? 1 : d->sequences, d->length, d->C, d->dtype, true))) return rc;
   if (!d->C || !d->sequences) return 0;
   if (d->length && !y) return fail(c, B200CONV_E_INVALID, "causal convolution without output");
   if (!d->length && !final) return 0;
@@ -3507,10 +3521,10 @@ int b200conv_causal_conv_grad(b200conv_ctx* c, const b200conv_causal_desc* d, co
   if (!c) return B200CONV_E_INVALID;
   std::lock_guard<std::mutex> g(c->mu);
   DeviceGuard dg(c->device);
-  int rc = check_causal(c, d, x, w, starts);
-  if (rc) return rc;
+  int rc = check_causal(c, d, x, w, bias, initial, dinitial, starts);
+  if (rc || (rc = check_aligned(c, {dw, dbias}, d->param_f32 ? 4 : row_elem_size(d->dtype)))) return rc;
   const long long n = d->packed ? 1 : d->sequences;
-  if ((rc = check_rows(c, "dy", dy, d->dy, n, d->length, d->C)) || (rc = check_rows(c, "dx", dx, d->dx, n, d->length, d->C, true))) return rc;
+  if ((rc = check_rows(c, "dy", dy, d->dy, n, d->length, d->C, d->dtype)) || (rc = check_rows(c, "dx", dx, d->dx, n, d->length, d->C, d->dtype, true))) return rc;
   const size_t ps = d->param_f32 ? 4 : row_elem_size(d->dtype);
   if (!d->C) return 0;
   if (!d->sequences || !d->length) {                // sums over no tokens
@@ -3539,8 +3553,8 @@ int b200conv_causal_conv_step(b200conv_ctx* c, const b200conv_causal_desc* d, co
   std::lock_guard<std::mutex> g(c->mu);
   DeviceGuard dg(c->device);
   if (d && (d->length != 1 || d->packed)) return fail(c, B200CONV_E_INVALID, "a step takes one token of every sequence");
-  int rc = check_causal(c, d, x, w, nullptr);
-  if (rc || (rc = check_rows(c, "y", y, d->y, d->sequences, 1, d->C, true))) return rc;
+  int rc = check_causal(c, d, x, w, bias, state, nullptr, nullptr);
+  if (rc || (rc = check_rows(c, "y", y, d->y, d->sequences, 1, d->C, d->dtype, true))) return rc;
   if (!d->C || !d->sequences) return 0;
   if (!state || !y) return fail(c, B200CONV_E_INVALID, "causal convolution step without state or output");
   CausalArgs a = {};
@@ -3551,25 +3565,27 @@ int b200conv_causal_conv_step(b200conv_ctx* c, const b200conv_causal_desc* d, co
 }
 
 static int check_scan(b200conv_ctx* c, const b200conv_scan_desc* d, const void* x, const void* dt, const float* A, const void* B, const void* C, const void* z,
-                      const int32_t* starts) {
+                      const int32_t* starts, std::initializer_list<const void*> f32) {
   if (!d) return fail(c, B200CONV_E_INVALID, "null descriptor");
   const long long n = d->packed ? 1 : d->sequences;
   int rc = check_sizes(c, n, d->length, d->C, d->dtype);
   if (rc) return rc;
   if (d->sequences < 0 || d->sequences > INT32_MAX / 8) return fail(c, B200CONV_E_INVALID, "%lld sequences", (long long)d->sequences);
   if (d->N < 1 || d->N > 128) return fail(c, B200CONV_E_UNSUPPORTED, "a selective scan has 1 to 128 states per channel, not %d", d->N);
+  if (1LL * d->groups * d->N > INT32_MAX / 2) return fail(c, B200CONV_E_UNSUPPORTED, "%d groups of %d states", d->groups, d->N);
   if (d->groups < 1 || d->C % d->groups) return fail(c, B200CONV_E_INVALID, "%d channels in %d groups", d->C, d->groups);
   if (d->packed && !starts) return fail(c, B200CONV_E_INVALID, "packed sequences without their offsets");
   if (!d->C || !d->sequences) return 0;
   if (!A) return fail(c, B200CONV_E_INVALID, "selective scan without A");
+  if ((rc = check_aligned(c, {A, starts}, 4)) || (rc = check_aligned(c, f32, 4))) return rc;
   if (d->length && (!x || !dt || !B || !C)) return fail(c, B200CONV_E_INVALID, "selective scan without x, dt, B or C");
   if (d->y.stored > d->C || d->dx.stored > d->C || d->ddt.stored > d->C || d->dz.stored > d->C)
     return fail(c, B200CONV_E_UNSUPPORTED, "a selective scan writes no pad channels");
   const int gn = d->groups * d->N;
-  if ((rc = check_rows(c, "x", x, d->x, n, d->length, d->C)) || (rc = check_rows(c, "dt", dt, d->dt, n, d->length, d->C)) ||
-      (rc = check_rows(c, "z", z, d->z, n, d->length, d->C)) || (rc = check_rows(c, "B", B, d->B, n, d->length, gn)))
+  if ((rc = check_rows(c, "x", x, d->x, n, d->length, d->C, d->dtype)) || (rc = check_rows(c, "dt", dt, d->dt, n, d->length, d->C, d->dtype)) ||
+      (rc = check_rows(c, "z", z, d->z, n, d->length, d->C, d->dtype)) || (rc = check_rows(c, "B", B, d->B, n, d->length, gn, d->dtype)))
     return rc;
-  return check_rows(c, "C", C, d->Cm, n, d->length, gn);
+  return check_rows(c, "C", C, d->Cm, n, d->length, gn, d->dtype);
 }
 
 int b200conv_selective_scan(b200conv_ctx* c, const b200conv_scan_desc* d, const void* x, const void* dt, const float* A, const void* B, const void* C,
@@ -3577,8 +3593,8 @@ int b200conv_selective_scan(b200conv_ctx* c, const b200conv_scan_desc* d, const 
   if (!c) return B200CONV_E_INVALID;
   std::lock_guard<std::mutex> g(c->mu);
   DeviceGuard dg(c->device);
-  int rc = check_scan(c, d, x, dt, A, B, C, z, starts);
-  if (rc || (rc = check_rows(c, "y", y, d->y, d->packed ? 1 : d->sequences, d->length, d->C, true))) return rc;
+  int rc = check_scan(c, d, x, dt, A, B, C, z, starts, {D, dt_bias, initial, final});
+  if (rc || (rc = check_rows(c, "y", y, d->y, d->packed ? 1 : d->sequences, d->length, d->C, d->dtype, true))) return rc;
   if (!d->C || !d->sequences) return 0;
   if (d->length && !y) return fail(c, B200CONV_E_INVALID, "selective scan without output");
   const size_t state_bytes = sizeof(float) * static_cast<size_t>(d->sequences) * d->C * d->N;
@@ -3620,14 +3636,14 @@ int b200conv_selective_scan_grad(b200conv_ctx* c, const b200conv_scan_desc* d, c
   if (!c) return B200CONV_E_INVALID;
   std::lock_guard<std::mutex> g(c->mu);
   DeviceGuard dg(c->device);
-  int rc = check_scan(c, d, x, dt, A, B, C, z, starts);
+  int rc = check_scan(c, d, x, dt, A, B, C, z, starts, {D, dt_bias, initial, dfinal, dA, dD, ddt_bias, dinitial});
   if (rc) return rc;
   if (!d->C) return 0;
   const long long n = d->packed ? 1 : d->sequences;
   const int gn = d->groups * d->N;
-  if ((rc = check_rows(c, "dy", dy, d->dy, n, d->length, d->C)) || (rc = check_rows(c, "dx", dx, d->dx, n, d->length, d->C, true)) ||
-      (rc = check_rows(c, "ddt", ddt, d->ddt, n, d->length, d->C, true)) || (rc = check_rows(c, "dz", dz, d->dz, n, d->length, d->C, true)) ||
-      (rc = check_rows(c, "dB", dB, d->dB, n, d->length, gn, true)) || (rc = check_rows(c, "dC", dC, d->dCm, n, d->length, gn, true)))
+  if ((rc = check_rows(c, "dy", dy, d->dy, n, d->length, d->C, d->dtype)) || (rc = check_rows(c, "dx", dx, d->dx, n, d->length, d->C, d->dtype, true)) ||
+      (rc = check_rows(c, "ddt", ddt, d->ddt, n, d->length, d->C, d->dtype, true)) || (rc = check_rows(c, "dz", dz, d->dz, n, d->length, d->C, d->dtype, true)) ||
+      (rc = check_rows(c, "dB", dB, d->dB, n, d->length, gn, d->dtype, true)) || (rc = check_rows(c, "dC", dC, d->dCm, n, d->length, gn, d->dtype, true)))
     return rc;
   if (!dA) return fail(c, B200CONV_E_INVALID, "selective scan gradient without dA");
   if (!z && dz) return fail(c, B200CONV_E_INVALID, "selective scan gradient with dz but without z");
@@ -3674,14 +3690,16 @@ int b200conv_selective_scan_step(b200conv_ctx* c, const b200conv_scan_desc* d, c
   std::lock_guard<std::mutex> g(c->mu);
   DeviceGuard dg(c->device);
   if (d && (d->length != 1 || d->packed)) return fail(c, B200CONV_E_INVALID, "a step takes one token of every sequence");
-  int rc = check_scan(c, d, x, dt, A, B, C, z, nullptr);
-  if (rc || (rc = check_rows(c, "y", y, d->y, d->sequences, 1, d->C, true))) return rc;
+  int rc = check_scan(c, d, x, dt, A, B, C, z, nullptr, {D, dt_bias, state});
+  if (rc || (rc = check_rows(c, "y", y, d->y, d->sequences, 1, d->C, d->dtype, true))) return rc;
   if (!d->C || !d->sequences) return 0;
   if (!state || !y) return fail(c, B200CONV_E_INVALID, "selective scan step without state or output");
   ScanArgs a = {};
   a.d = *d;
   a.x = x; a.dt = dt; a.A = A; a.B = B; a.C = C; a.D = D; a.z = z; a.dt_bias = dt_bias; a.final = state; a.y = y;
-  KLAUNCH(c, kKScan, launch_scan_step(a, c->stream));
+  int launches = 0;
+  KLAUNCH(c, kKScan, launch_scan_step(a, &launches, c->stream));
+  count_launches(c, launches - 1);
   return 0;
 }
 

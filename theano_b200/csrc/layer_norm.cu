@@ -430,12 +430,12 @@ cudaError_t backward(const NormArgs& a, int* launches, cudaStream_t s) {
     if (vecs <= 256) B200_NORM(2, 128)
     if (vecs <= 512) B200_NORM(2, 256)
     if (vecs <= 1024) B200_NORM(2, 512)
-    launch_streaming(norm_grad_long_kernel<T>, static_cast<unsigned>(rows), 512, 0, s, a);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    if (a.partial) {
+    if (a.partial) {                             // first: dx may lie over dy
       launch_streaming(norm_grad_columns_kernel<T>, dim3((a.d.C + 255) / 256, parts), 256, 0, s, a);
+      if ((e = cudaGetLastError()) != cudaSuccess) return e;
       ++*launches;
     }
+    launch_streaming(norm_grad_long_kernel<T>, static_cast<unsigned>(rows), 512, 0, s, a);
   } while (0);
 #undef B200_NORM
   if ((e = cudaGetLastError()) != cudaSuccess || !a.partial) return e;

@@ -290,7 +290,7 @@ cudaError_t launch_selective_scan(const ScanArgs& a, int* launches, cudaStream_t
 }
 
 template <typename T, int P, bool QUADS>
-cudaError_t run_step(const ScanArgs& a, cudaStream_t s) {
+cudaError_t run_step(const ScanArgs& a, int* launches, cudaStream_t s) {
   const int wide = kStepThreads / P;
   const unsigned blocks = static_cast<unsigned>((a.d.C + wide - 1) / wide);
   for (int64_t first = 0; first < a.d.sequences; first += 65535) {
@@ -301,26 +301,28 @@ cudaError_t run_step(const ScanArgs& a, cudaStream_t s) {
     b.y = const_cast<T*>(on(a.y, a.d.y.seq));
     b.final = a.final + first * a.d.C * a.d.N;
     launch_streaming(scan_step_kernel<T, P, QUADS>, dim3(blocks, n), kStepThreads, 0, s, b);
+    ++*launches;
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
 }
 template <typename T>
-cudaError_t run_step_type(const ScanArgs& a, cudaStream_t s) {
+cudaError_t run_step_type(const ScanArgs& a, int* launches, cudaStream_t s) {
   const int N = a.d.N;
   const size_t quad = 4 * sizeof(T);
   auto whole = [&](const void* p, const b200conv_rows& r) { return reinterpret_cast<uintptr_t>(p) % quad == 0 && r.seq * sizeof(T) % quad == 0; };
   const bool quads = N % 4 == 0 && aligned16({a.final, a.A}) && whole(a.B, a.d.B) && whole(a.C, a.d.Cm);
-#define B200_LANES(P) if (N <= 8 * P) return quads ? run_step<T, P, true>(a, s) : run_step<T, P, false>(a, s);
+#define B200_LANES(P) if (N <= 8 * P) return quads ? run_step<T, P, true>(a, launches, s) : run_step<T, P, false>(a, launches, s);
   B200_LANES(1) B200_LANES(2) B200_LANES(4) B200_LANES(8) B200_LANES(16)
 #undef B200_LANES
   return cudaErrorInvalidValue;
 }
 
-cudaError_t launch_scan_step(const ScanArgs& a, cudaStream_t s) {
-  if (a.d.dtype == B200CONV_F32) return run_step_type<float>(a, s);
-  return a.d.dtype == B200CONV_F16 ? run_step_type<__half>(a, s) : run_step_type<__nv_bfloat16>(a, s);
+cudaError_t launch_scan_step(const ScanArgs& a, int* launches, cudaStream_t s) {
+  *launches = 0;
+  if (a.d.dtype == B200CONV_F32) return run_step_type<float>(a, launches, s);
+  return a.d.dtype == B200CONV_F16 ? run_step_type<__half>(a, launches, s) : run_step_type<__nv_bfloat16>(a, launches, s);
 }
 
 int scan_state_slots(int N) { return N <= 8 ? 8 : N <= 16 ? 16 : N <= 32 ? 32 : N <= 64 ? 64 : 128; }
@@ -338,6 +340,7 @@ void cut_pieces(ScanArgs* a, long long tiles, long long slots) {
     if (m > 1 && size < 32) break;
     // packed: windows of `size` rows, and a piece more for each sequence that begins inside of one
     const long long blocks = tiles * (a->d.packed ? length / size + sequences : sequences * ((length + size - 1) / size));
+    if (m > 1 && blocks > 3 * slots) break;
     // a cut sequence is walked twice, the first time for its ends alone
     const long long cost = (blocks + slots - 1) / slots * (size + kStart) * (m > 1 ? 7 : 4);
     if (best < 0 || cost < best) {

@@ -65,6 +65,6 @@ void plan_grad_pieces(ScanArgs* a);
 int scan_grad_slots(int N);              // the same in those of the gradient
 long long scan_kept(const ScanArgs& a);    // kept states per channel
 cudaError_t launch_scan_grad(const ScanArgs& a, int* launches, cudaStream_t s);
-cudaError_t launch_scan_step(const ScanArgs& a, cudaStream_t s);
+cudaError_t launch_scan_step(const ScanArgs& a, int* launches, cudaStream_t s);
 
 }  // namespace b200
