@@ -292,9 +292,9 @@ int b200conv_causal_conv_step(b200conv_ctx* ctx, const b200conv_causal_desc* d, 
  * first (NULL: zeros) and behind the last token; they may be one array.  Packed sequences as above; `longest` is an upper bound of their
  * lengths that only guides the cut of the work (0: not known).
  * The gradient takes the forward call's inputs, dy and, where given, dfinal (like final), and writes dx, ddt, dA, dB, dC, dz (with z), and
- * where given dD, ddt_bias and dinitial (like initial); rows of no sequence are left as they were.  Its workspace is one float32 state per
- * eight tokens and channel and, for every 4 * floor(128 / L) channels of a group (L: lanes of a channel, 4 up to N = 16, 8, 16, 32 up to
- * N = 128), one pair of float32 B and C rows per token.
+ * where given dD, ddt_bias and dinitial (like initial, may be dfinal); rows of no sequence are left as they were.  Its workspace is the
+ * float32 states of every channel for each fourth token and, for every 2048 / N' channels of a group (N': N rounded up to 16, 32, 64 or
+ * 128), one pair of float32 B and C rows per token.
  * The step takes one token of every sequence (length 1) and moves `state`, like initial, on in place; y may be x, dt or z. */
 typedef struct b200conv_scan_desc {
   int64_t sequences, length;
@@ -362,7 +362,7 @@ long long b200conv_launch_count(b200conv_ctx* ctx);
  * CUDA events on the context's stream; b200conv_kernel_time() then returns the summed duration
  * and the launch count of one kernel family since timing was enabled: "conv_umma" (forward and
  * gradInputs main kernel), "conv_reduce" (its second half when the reduction is split over CTAs), "wgrad_umma",
- * "wgrad_reduce", "transpose", "pack", "direct", "pool". */
+ * "wgrad_reduce", "transpose", "pack", "direct", "pool", and of the sequence operators "layer_norm", "causal_conv", "selective_scan". */
 int b200conv_kernel_timing(b200conv_ctx* ctx, int enable);
 int b200conv_kernel_time(b200conv_ctx* ctx, const char* family, float* total_ms, int* launches);
 /* Forward and gradInputs have two tensor-core kernels (activations fetched once per channel

@@ -4,8 +4,11 @@
 //
 // (a true convolution; without `flip` the taps are counted from the oldest token).  Tokens before a sequence's first are
 // the rows of its initial state, or zeros; the final state is the last taps - 1 rows of (initial state, x).
-// HBM bound: x is read once, y written once.  A thread takes V neighbouring channels (16 bytes) and walks along a run of
-// tokens with the last taps - 1 rows in registers; only those rows are read a second time, out of L2, by the next run.
+// x is read once and y written once: a thread takes four neighbouring channels and walks along a run of tokens with the last taps - 1 rows
+// in registers; only those rows are read a second time, out of L2, by the next run.  Runs are as long as lets all blocks be
+// resident at once, and the rows ahead are loaded while the present ones are computed.  8192 packed tokens of 2048 channels,
+// 4 taps, bfloat16: 21 us (3.2 TB/s), bound by the issue slots and the special function unit together (18 instructions per element and
+// lane, two trips for SiLU); with 8 channels per thread 33 us, without rows on their way 37.  4 x 2047 x 1024 float32: 12 us (5.6 TB/s).
 #include "causal_conv.cuh"
 #include "internal.h"
 
@@ -95,7 +98,8 @@ __global__ void __launch_bounds__(256, kBlocks<T, K>) causal_conv_kernel(CausalA
   }
 }
 
-// One token of every sequence: reads the state and the token, leaves y and the state moved on by a row.
+// One token of every sequence: reads the state and the token, leaves y and the state moved on by a row.  64 x 2048 bfloat16: 3.9 us, the
+// time of a launch and two trips to memory (2.1 MB); eight channels per thread, so that a row of the state is one load.
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(128) causal_step_kernel(CausalArgs a, int vecs) {
   pdl_enter();

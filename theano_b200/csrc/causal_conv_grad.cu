@@ -3,10 +3,11 @@
 //   g[t] = dy[t] silu'(pre[t])  (pre from x again),   dx[t] = sum over k of w[k] g[t + k],
 //   dw[k] = sum over tokens of g[t] x[t - k],  dbias = sum of g,  and the initial state's rows like tokens before the first
 //
-// HBM bound: x and dy are read once, dx is written once.  A thread walks along a run of tokens with the last taps - 1 rows of x
-// and the unfinished sums of dx in registers, and taps - 1 tokens beyond its run for the sums that end there.  The
-// filters' sums stay in registers too; a block adds its runs and leaves one row of partial sums, which a second kernel adds
-// in block order.
+// x and dy are read once, dx is written once.  A thread walks along a run of tokens with the last taps - 1 rows of x and the unfinished sums
+// of dx in registers, and taps - 1 tokens beyond its run for the sums that end there.  The filters' sums stay in registers too; a
+// block adds its runs and leaves one row of partial sums, which a second kernel adds in block order.  4 x 2047 x 1024 float32, 4 taps:
+// 25 us (4.0 TB/s) and 5 for the second kernel; four channels per thread take 166 registers, three blocks of 128 threads to an SM, which
+// bounds the bytes on their way.  Blocks of 256 threads left one to an SM: 45 us.
 #include "causal_conv.cuh"
 #include "internal.h"
 
