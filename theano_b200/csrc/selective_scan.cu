@@ -18,13 +18,17 @@ namespace {
 // is shared by all of them; the rows of B and C, the same for all lanes, come from shared memory as float32.
 constexpr int kScanBlocks = 4;                   // of an SM: 16 warps, 128 registers a thread
 
-template <typename T, int S, int P, bool WIDE, bool LOCAL>
+// ASYNC: x, dt and z of 16-bit tensors on their boundaries come by asynchronous copies, a tile ahead, in 16 bytes (182 us, by loads
+// of two bytes per lane 190: no addresses per token, no registers for tokens on their way).
+template <typename T, int S, int P, bool WIDE, bool LOCAL, bool ASYNC>
 __global__ void __launch_bounds__(kScanThreads, S * P <= 32 ? kScanBlocks : 1) scan_lane_kernel(ScanArgs a) {
-  constexpr int NS = S * P, kWide = kScanThreads / P, kTokens = tile_tokens(NS);
+  constexpr int NS = S * P, kWide = kScanThreads / P, kTokens = ASYNC && NS <= 32 ? 16 : tile_tokens(NS);
   constexpr int kGroup = LOCAL ? 8 : 4;          // tokens whose x, dt and z a lane has in flight
-  using Rows = StateRows<T, NS, WIDE, !LOCAL>;
+  using Rows = StateRows<T, NS, WIDE, !LOCAL, kTokens>;
   pdl_enter();
   __shared__ __align__(16) float st[2][(LOCAL ? 1 : 2) * kTokens * NS];
+  constexpr int kArrays = LOCAL ? 2 : 3;
+  __shared__ __align__(16) T rows_in[ASYNC ? 2 : 1][ASYNC ? kArrays : 1][ASYNC ? kTokens : 1][ASYNC ? kWide : 8];
   const int id = blockIdx.x / a.tiles;
   const ScanTile ct = scan_tile(a, blockIdx.x - id * a.tiles, kWide);
   const Piece p = piece_of(a, id);
@@ -66,7 +70,27 @@ __global__ void __launch_bounds__(kScanThreads, S * P <= 32 ? kScanBlocks : 1) s
   const T* B = static_cast<const T*>(a.B) + p.base * a.d.B.seq + 1LL * ct.group * N;
   const T* C = static_cast<const T*>(a.C) + p.base * a.d.Cm.seq + 1LL * ct.group * N;
   T nx[kGroup], nd[kGroup], nz[kGroup];
+  auto copy_tile = [&](long long tile, int turn) {
+    if constexpr (ASYNC) {
+      constexpr int kVec = 16 / sizeof(T), kRow = kWide / kVec;
+      const int n = p.to - tile < kTokens ? static_cast<int>(p.to - tile) : kTokens;
+#pragma unroll
+      for (int w = 0; w < kArrays; ++w) {
+        const void* base = w == 0 ? a.x : w == 1 ? a.dt : a.z;
+        const b200conv_rows& r = w == 0 ? a.d.x : w == 1 ? a.d.dt : a.d.z;
+        if (!base) continue;
+        const T* src = static_cast<const T*>(base) + p.base * r.seq + tile * r.row + ct.channel;
+#pragma unroll
+        for (int i = threadIdx.x; i < kTokens * kRow; i += kScanThreads) {
+          const int t = i / kRow, cc = i % kRow * kVec;
+          if (t < n && cc < ct.channels) copy_async(&rows_in[turn][w][t][cc], src + t * r.row + cc);
+        }
+      }
+      copies_issued();
+    }
+  };
   auto fetch = [&](int left) {                   // the next tokens of the piece, of which there are `left`
+    if (ASYNC) return;
     if (left >= kGroup) {
 #pragma unroll
       for (int k = 0; k < kGroup; ++k) {
@@ -92,12 +116,21 @@ __global__ void __launch_bounds__(kScanThreads, S * P <= 32 ? kScanBlocks : 1) s
   Rows rows;
   rows.load(B, a.d.B.row, C, a.d.Cm.row, p.from, p.to, N);
   int left = static_cast<int>(p.to - p.from);    // tokens that have not been fetched
+  if (ASYNC) copy_tile(p.from, 0);
   fetch(left);
   left -= kGroup;
   float sum = 0.f;
   int turn = 0;
-  // kGroup tokens from shared memory at `at`; `live`: how many of them belong to the piece
-  auto group = [&](const float* at, int live, auto whole) {
+  // kGroup tokens from shared memory at `at`, the tile's from t0 on; `live`: how many of them belong to the piece
+  auto group = [&](const float* at, int t0, int live, auto whole) {
+    if constexpr (ASYNC) {
+#pragma unroll
+      for (int k = 0; k < kGroup; ++k) {
+        nx[k] = rows_in[turn][0][t0 + k][ch];
+        nd[k] = rows_in[turn][1][t0 + k][ch];
+        if (!LOCAL && a.z) nz[k] = rows_in[turn][kArrays - 1][t0 + k][ch];
+      }
+    }
     float xv[kGroup], zv[kGroup], d[kGroup], u[kGroup];
 #pragma unroll
     for (int k = 0; k < kGroup; ++k) {
@@ -147,13 +180,15 @@ __global__ void __launch_bounds__(kScanThreads, S * P <= 32 ? kScanBlocks : 1) s
   };
   for (long long tile = p.from; tile < p.to; tile += kTokens, turn ^= 1) {
     rows.store(st[turn]);
+    if (ASYNC) copies_landed();
     __syncthreads();                             // the tile is there, and the one before the last has been read
+    if (ASYNC && tile + kTokens < p.to) copy_tile(tile + kTokens, turn ^ 1);
     rows.load(B, a.d.B.row, C, a.d.Cm.row, tile + kTokens, p.to, N);
     const int n = p.to - tile < kTokens ? static_cast<int>(p.to - tile) : kTokens;
     const float* at = st[turn] + q * S;
     int t0 = 0;
-    for (; t0 + kGroup <= n; t0 += kGroup) group(at + t0 * NS, kGroup, std::true_type());
-    if (t0 < n) group(at + t0 * NS, n - t0, std::false_type());
+    for (; t0 + kGroup <= n; t0 += kGroup) group(at + t0 * NS, t0, kGroup, std::true_type());
+    if (t0 < n) group(at + t0 * NS, t0, n - t0, std::false_type());
   }
   if (!mine) return;
   if (LOCAL) {
@@ -258,7 +293,7 @@ __global__ void __launch_bounds__(kStepThreads) scan_step_kernel(ScanArgs a) {
 
 }  // namespace
 
-template <typename T, int S, int P, bool WIDE>
+template <typename T, int S, int P, bool WIDE, bool ASYNC>
 cudaError_t run_lanes(ScanArgs a, int* launches, cudaStream_t s) {
   const int wide = kScanThreads / P, per = a.d.C / a.d.groups;
   a.tiles = a.d.groups * ((per + wide - 1) / wide);
@@ -266,19 +301,27 @@ cudaError_t run_lanes(ScanArgs a, int* launches, cudaStream_t s) {
   if (grid >= INT32_MAX) return cudaErrorInvalidValue;
   *launches = 1;
   if (a.piece_state) {
-    launch_streaming(scan_lane_kernel<T, S, P, WIDE, true>, static_cast<unsigned>(grid), kScanThreads, 0, s, a);
+    launch_streaming(scan_lane_kernel<T, S, P, WIDE, true, ASYNC>, static_cast<unsigned>(grid), kScanThreads, 0, s, a);
     ++*launches;
     const cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
   }
-  launch_streaming(scan_lane_kernel<T, S, P, WIDE, false>, static_cast<unsigned>(grid), kScanThreads, 0, s, a);
+  launch_streaming(scan_lane_kernel<T, S, P, WIDE, false, ASYNC>, static_cast<unsigned>(grid), kScanThreads, 0, s, a);
   return cudaGetLastError();
 }
 template <typename T>
 cudaError_t run_type(const ScanArgs& a, int* launches, cudaStream_t s) {
   const int N = a.d.N;
   const bool wide = N % (16 / sizeof(T)) == 0 && rows_aligned(a.B, a.d.B, a.d.dtype) && rows_aligned(a.C, a.d.Cm, a.d.dtype);
-#define B200_LANES(S, P) if (N <= S * P) return wide ? run_lanes<T, S, P, true>(a, launches, s) : run_lanes<T, S, P, false>(a, launches, s);
+  // channels of a block in whole 16-byte pieces
+  const bool async = sizeof(T) == 2 && N <= 32 && wide && a.d.C / a.d.groups % 8 == 0 && rows_aligned(a.x, a.d.x, a.d.dtype) &&
+                     rows_aligned(a.dt, a.d.dt, a.d.dtype) && rows_aligned(a.z, a.d.z, a.d.dtype);
+  if constexpr (sizeof(T) == 2) {
+    if (async && N <= 8) return run_lanes<T, 8, 1, true, true>(a, launches, s);
+    if (async && N <= 16) return run_lanes<T, 16, 1, true, true>(a, launches, s);
+    if (async) return run_lanes<T, 16, 2, true, true>(a, launches, s);
+  }
+#define B200_LANES(S, P) if (N <= S * P) return wide ? run_lanes<T, S, P, true, false>(a, launches, s) : run_lanes<T, S, P, false, false>(a, launches, s);
   B200_LANES(8, 1) B200_LANES(16, 1) B200_LANES(16, 2) B200_LANES(16, 4) B200_LANES(16, 8)
 #undef B200_LANES
   return cudaErrorInvalidValue;

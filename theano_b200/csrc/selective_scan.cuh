@@ -131,10 +131,20 @@ __device__ __forceinline__ void clear_piece_sums(const ScanArgs& a, int id, cons
 constexpr int kPolyPairs = 1;                    // pairs of decays that a lane takes by polynomial: none 227, one 210, two 216 us (8192 tokens, 2048 channels)
 constexpr int tile_tokens(int NS) { return NS <= 32 ? 32 : 1024 / NS; }           // of a tile of B and C
 
+// 16 bytes from global to shared memory without a register in between.
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async_4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_landed() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // Rows of B (and C) of a tile on their way to shared memory: [B or C][tokens][NS], zeros beyond N and beyond the piece.
-template <typename T, int NS, bool WIDE, bool BOTH>
+template <typename T, int NS, bool WIDE, bool BOTH, int TOKENS = tile_tokens(NS)>
 struct StateRows {
-  static constexpr int kTokens = tile_tokens(NS), kVec = WIDE ? 16 / sizeof(T) : 1, kRow = NS / kVec, kAll = (BOTH ? 2 : 1) * kTokens * kRow,
+  static constexpr int kTokens = TOKENS, kVec = WIDE ? 16 / sizeof(T) : 1, kRow = NS / kVec, kAll = (BOTH ? 2 : 1) * kTokens * kRow,
                        kMine = (kAll + kScanThreads - 1) / kScanThreads;
   Pack<T, kVec> v[kMine];
   __device__ __forceinline__ void load(const T* B, long long brow, const T* C, long long crow, long long tok, long long to, int N) {

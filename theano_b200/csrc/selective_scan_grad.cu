@@ -162,16 +162,6 @@ __global__ void __launch_bounds__(kScanThreads, S * P <= 32 ? (CUT ? 3 : 4) : 1)
   if (q == 0) a.piece_sum[1LL * id * a.d.C + c] = sum;
 }
 
-// 16 bytes from global to shared memory without a register in between.
-__device__ __forceinline__ void copy_async(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy_async_4(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void copies_landed() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
 // Shared memory of the backward walk.
 template <typename T, int P, bool CUT> struct GradShape {
   static constexpr int NS = 16 * P, kWide = kScanThreads / P, kWarps = kScanThreads / 32;
