@@ -135,3 +135,26 @@ def test_same_bits_every_time_and_in_a_graph():
     other.launch()
     graph.launch()
     assert all(np.array_equal(first[k], t.to_host()) for k, t in grads.items())
+
+
+@pytest.mark.parametrize("T", [8, 300])
+@pytest.mark.parametrize("C,N,G", [(48, 16, 3), (10, 40, 1), (4, 16, 1)])
+def test_nothing_of_an_earlier_call_is_left(T, C, N, G):
+    """Blocks with fewer channels than lanes, behind calls that filled every SM's shared memory with NaN: the sums over channels
+    hold nothing of what lies there."""
+    ctx = shim.get_context(0)
+    f32 = np.dtype(np.float32)
+    v = inputs(3, [T] * 2, C, N, G, f32)
+    dev = lambda k: put(ctx, np.stack(v[k]), f32)  # noqa: E731
+    args = (dev("x"), dev("x"), dev("dt"), put(ctx, v["A"], f32), dev("B"), dev("C"))
+    want = plain(v, (), True, dys=v["x"])
+    m = plain(v, (), True, dys=v["x"], magnitudes=True)
+    nan = lambda *s: put(ctx, np.full(s, np.nan), f32)  # noqa: E731
+    wide = (nan(300, 16, 128), nan(300, 16, 128), nan(300, 16, 128), nan(128, 16), nan(300, 16, 16), nan(300, 16, 16))
+    for _ in range(3):
+        Q.device_selective_scan(*wide[1:], softplus=True)
+        Q.device_selective_scan_grad(*wide, softplus=True)
+        got = Q.device_selective_scan_grad(*args, softplus=True)
+        for k in ("x", "dt", "B", "C"):
+            close(got[k].to_host(), np.stack(want["d" + k]), f32, sums(v) * E32 * np.stack(m["d" + k]))
+        close(got["A"].to_host(), want["dA"], f32, sums(v) * E32 * m["dA"])

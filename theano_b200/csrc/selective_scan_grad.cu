@@ -343,6 +343,13 @@ __global__ void __launch_bounds__(kScanThreads, P == 1 ? kGradBlocks : 1) scan_g
       states[k] = m < N && t < n ? k < kMine / 2 ? B[(tok + t) * a.d.B.row + m] : C[(tok + t) * a.d.Cm.row + m] : from_float<T>(0.f);
     }
   };
+  if (!mine)                                     // lanes without a channel take part in the sums over channels: as zeros
+#pragma unroll
+    for (int k = 0; k < 2 * (kStep / kKeep); ++k) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) sh.kept[k / (kStep / kKeep)][k % (kStep / kKeep)][s][threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (CUT) sh.kept_sum[k / (kStep / kKeep)][k % (kStep / kKeep)][ch] = 0.f;
+    }
   int turn = 0;
   if (steps > 0) {
     load_tile(last, 0);
