@@ -128,7 +128,7 @@ __device__ __forceinline__ void clear_piece_sums(const ScanArgs& a, int id, cons
     a.partial_d[2LL * id * a.d.C + ct.channel + i] = a.partial_d[(2LL * id + 1) * a.d.C + ct.channel + i] = 0.f;
 }
 
-constexpr int kPolyPairs = 1;                    // pairs of decays that a lane takes by polynomial: none 227, one 210, two 216 us (8192 tokens, 2048 channels)
+constexpr int kPolyPairs = 1;                    // pairs of decays that a lane takes by polynomial: none 227, one 210, two 216 us when it was brought (8192 tokens, 2048 channels), two against one 196 to 190 us since
 constexpr int tile_tokens(int NS) { return NS <= 32 ? 32 : 1024 / NS; }           // of a tile of B and C
 
 // 16 bytes from global to shared memory without a register in between.
