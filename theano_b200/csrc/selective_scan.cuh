@@ -29,12 +29,20 @@ __device__ __forceinline__ float softplus(float v) {
   q = fmaf(q, e, 0.9999999403953552f);
   return fmaf(q, e, fmaxf(v, 0.f));
 }
+// v held between -127 and 128; NaN stays NaN.
+__device__ __forceinline__ float clamp_exponent(float v) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(-127.f));
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(r), "f"(128.f));
+  return r;
+}
 // 2^v of both without the special function unit: v = n + f with n the nearest integer (the low bits of v + 1.5 * 2^23), 2^f a
 // polynomial of degree 5 fitted here by iteratively reweighted least squares (off by 2e-7 with float32 roundings), 2^n into the
-// exponent.  Arguments from -126 on (below: 2^-126) up to 127.
+// exponent.  The ends of the range come out of the same addition: 2^128 is the infinity's bits, 2^-127 those of zero (between 2^-127 and
+// 2^-126 results are off by up to 2^-127).  The addition makes a number of a NaN's bits: v * 0 brings it back.
 __device__ __forceinline__ Pair exp2_poly(Pair a) {
   const float2 v = a.get();
-  const Pair x(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f)), magic(12582912.f, 12582912.f), back(-12582912.f, -12582912.f), minus(-1.f, -1.f);
+  const Pair x(clamp_exponent(v.x), clamp_exponent(v.y)), magic(12582912.f, 12582912.f), back(-12582912.f, -12582912.f), minus(-1.f, -1.f);
   const Pair t = add2(x, magic), f = fma2(add2(t, back), minus, x);
   Pair p = fma2(f, Pair(0.001326472731307149f, 0.001326472731307149f), Pair(0.009671512991189957f, 0.009671512991189957f));
   p = fma2(p, f, Pair(0.05550733581185341f, 0.05550733581185341f));
@@ -42,7 +50,8 @@ __device__ __forceinline__ Pair exp2_poly(Pair a) {
   p = fma2(p, f, Pair(0.6931470036506653f, 0.6931470036506653f));
   p = fma2(p, f, Pair(1.f, 1.f));
   const float2 r = p.get(), n = t.get();
-  return Pair(__int_as_float(__float_as_int(r.x) + (__float_as_int(n.x) << 23)), __int_as_float(__float_as_int(r.y) + (__float_as_int(n.y) << 23)));
+  const Pair e(__int_as_float(__float_as_int(r.x) + (__float_as_int(n.x) << 23)), __int_as_float(__float_as_int(r.y) + (__float_as_int(n.y) << 23)));
+  return fma2(x, Pair(0.f, 0.f), e);
 }
 __device__ __forceinline__ Pair exp2_pair(Pair a) {
   const float2 f = a.get();
