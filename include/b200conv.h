@@ -294,7 +294,8 @@ int b200conv_causal_conv_step(b200conv_ctx* ctx, const b200conv_causal_desc* d, 
  * The gradient takes the forward call's inputs, dy and, where given, dfinal (like final), and writes dx, ddt, dA, dB, dC, dz (with z), and
  * where given dD, ddt_bias and dinitial (like initial, may be dfinal); rows of no sequence are left as they were.  Its workspace is the
  * float32 states of every channel for each fourth token and, for every 2048 / N' channels of a group (N': N rounded up to 16, 32, 64 or
- * 128), one pair of float32 B and C rows per token.
+ * 128), one pair of float32 B and C rows per token.  It multiplies the decays of stretches of tokens: where growing ones exceed float32
+ * together, gradients before and behind them may be infinite or NaN although their own sums would not be.
  * The step takes one token of every sequence (length 1) and moves `state`, like initial, on in place; y may be x, dt or z. */
 typedef struct b200conv_scan_desc {
   int64_t sequences, length;

@@ -2,7 +2,8 @@
 import numpy as np
 import pytest
 
-from sequence_util import DTYPES, put
+import sequence_plain as P
+from sequence_util import DTYPES, close, put
 from theano_b200 import sequence as Q
 from theano_b200 import shim
 
@@ -103,3 +104,24 @@ def test_gradients_behind_an_overflow(dt, C, N):
     A[2, 0] = np.nan
     dC = gradient(A)
     assert np.isnan(dC[:, 0]).all() and (dC[:at, 1:] == C).all()
+
+
+def test_states_of_zero_stay_zero_while_decays_grow():
+    """A prompt that begins with tokens of no input and large growing steps, long enough to be cut: a piece's decays together exceed float32,
+    the states do not."""
+    ctx = shim.get_context(0)
+    C, N, T, quiet = 8, 16, 400, 250
+    rs = np.random.RandomState(2)
+    x, steps = rs.standard_normal((T, C)).astype(np.float32), np.full((T, C), 2.0 ** -7, np.float32)
+    B, Cm = rs.standard_normal((2, T, 1, N)).astype(np.float32)
+    x[:quiet], steps[:quiet] = 0, 4
+    A = np.full((C, N), 1.0, np.float32)
+    want, m = (P.selective_scan([x], [steps], A, [B], [Cm], magnitudes=k) for k in (False, True))
+    # a path through the T - quiet tokens behind the growth (an exponential of 4 and three roundings of an argument below 1 each), their
+    # pieces' sums of deltas, sums over states
+    e = (60 + 7.4 * (T - quiet)) * 2.0 ** -24
+    for initial in (0.0, -0.0):
+        y, final = run(ctx, F32, x[None], steps[None], A, B[None], Cm[None], np.full((1, C, N), initial, np.float32))
+        assert (y[0, :quiet] == 0).all()
+        close(y[0], want["y"][0], F32, e * m["y"][0])
+        close(final, want["final"], F32, e * m["final"])

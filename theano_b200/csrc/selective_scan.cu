@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(kScanThreads, S * P <= 32 ? kScanBlocks : 1) s
   if (!LOCAL && mine)
 #pragma unroll 4
     for (int j = p.first; j < id; ++j) {         // what the pieces before this one made of it
-      const float all = a.piece_sum[1LL * j * a.d.C + c];
+      const float sum = a.piece_sum[1LL * j * a.d.C + c], all = any_of(h) ? sum : 0.f;
       const float4* f = reinterpret_cast<const float4*>(a.piece_state + (1LL * j * a.d.C + c) * NS + q * S);
 #pragma unroll
       for (int s = 0; s < S / 4; ++s) {

@@ -58,6 +58,15 @@ __device__ __forceinline__ Pair exp2_pair(Pair a) {
   return Pair(exp2_fast(f.x), exp2_fast(f.y));
 }
 
+// Whether a lane has a state that is not zero.  Where pieces are joined zeros are not multiplied by the decays of a whole piece: growing
+// ones may exceed float32 together where the tokens' own, one after the other, leave the zero alone.
+template <int M> __device__ __forceinline__ bool any_of(const Pair (&v)[M]) {
+  unsigned long long bits = 0;
+#pragma unroll
+  for (int s = 0; s < M; ++s) bits |= v[s].v;
+  return bits & 0x7fffffff7fffffffull;
+}
+
 // A log2(e).  A decay of minus infinity ends a state in any step of positive size and, like every other, not in one of size zero
 // (as which the tokens behind a piece count).
 __device__ __forceinline__ float scaled_decay(float A) {
