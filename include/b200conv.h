@@ -267,7 +267,7 @@ int b200conv_layer_norm_grad(b200conv_ctx* ctx, const b200conv_norm_desc* d, con
  * Packed sequences (`packed`): the tensors have `length` rows, sequence i takes rows starts[i] to starts[i + 1] - 1, with
  * sequences + 1 offsets in device memory that do not decrease and do not exceed length; sequences may be empty, rows of no
  * sequence are neither read nor written.  Offsets that break this give wrong results, no access outside of the tensors.
- * The gradient: dx, and where given dw and dbias (like w, bias) and dinitial (like initial).
+ * The gradient: dx, and where given dw and dbias (like w, bias) and dinitial (like initial, may be it).
  * The step takes one token of every sequence ([sequences][C]: length 1) and moves `state`, like initial, on in place. */
 typedef struct b200conv_causal_desc {
   int64_t sequences, length;
@@ -292,7 +292,7 @@ int b200conv_causal_conv_step(b200conv_ctx* ctx, const b200conv_causal_desc* d, 
  * first (NULL: zeros) and behind the last token; they may be one array.  Packed sequences as above; `longest` is an upper bound of their
  * lengths that only guides the cut of the work (0: not known).
  * The gradient takes the forward call's inputs, dy and, where given, dfinal (like final), and writes dx, ddt, dA, dB, dC, dz (with z), and
- * where given dD, ddt_bias and dinitial (like initial, may be dfinal); rows of no sequence are left as they were.  Its workspace is the
+ * where given dD, ddt_bias and dinitial (like initial, may be it or dfinal); rows of no sequence are left as they were.  Its workspace is the
  * float32 states of every channel for each fourth token and, for every 2048 / N' channels of a group (N': N rounded up to 16, 32, 64 or
  * 128), one pair of float32 B and C rows per token.  It multiplies the decays of stretches of tokens: where growing ones exceed float32
  * together, gradients before and behind them may be infinite or NaN although their own sums would not be.

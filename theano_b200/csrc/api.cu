@@ -3539,6 +3539,7 @@ int b200conv_causal_conv_grad(b200conv_ctx* c, const b200conv_causal_desc* d, co
   a.d = *d;
   a.dy = dy; a.x = x; a.w = w; a.bias = bias; a.initial = initial; a.starts = d->packed ? starts : nullptr;
   a.dx = dx; a.dw = dw; a.dbias = dbias; a.dinitial = dinitial;
+  if ((rc = detach_state(c, tmp, &a.initial, dinitial, causal_state_bytes(d)))) return rc;
   if ((dw || dbias) && (rc = tmp.get(sizeof(float) * (d->width + 1) * d->C * static_cast<size_t>(causal_grad_parts(a)),
                                      reinterpret_cast<void**>(&a.partial))))
     return rc;
@@ -3666,8 +3667,9 @@ int b200conv_selective_scan_grad(b200conv_ctx* c, const b200conv_scan_desc* d, c
   a.starts = d->packed ? starts : nullptr;
   a.dx = dx; a.ddt = ddt; a.dA = dA; a.dB = dB; a.dC = dC; a.dD = dD; a.dz = dz; a.ddt_bias = ddt_bias; a.dinitial = dinitial;
   plan_grad_pieces(&a);
-  const void* after = dfinal;
-  if ((rc = detach_state(c, tmp, &after, dinitial, state_bytes))) return rc;
+  const void *before = initial, *after = dfinal;
+  if ((rc = detach_state(c, tmp, &after, dinitial, state_bytes)) || (rc = detach_state(c, tmp, &before, dinitial, state_bytes))) return rc;
+  a.initial = static_cast<const float*>(before);
   a.dfinal = static_cast<const float*>(after);
   const size_t kept = static_cast<size_t>(scan_kept(a)) * d->C, slots = scan_grad_slots(d->N), pieces = static_cast<size_t>(a.pieces) * d->C;
   auto get = [&](size_t floats, float** p) { return tmp.get(sizeof(float) * floats, reinterpret_cast<void**>(p)); };
