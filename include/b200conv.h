@@ -232,8 +232,9 @@ int b200conv_channel_sum(b200conv_ctx* ctx, const void* x, void* out, long long 
  * pad channels of a channels-last image must hold; 0 or C writes nothing beyond C.
  *
  * An output may be an input of the same shape and strides where a call says so; otherwise outputs overlap neither inputs nor
- * each other (rows of two tensors may interleave: halves of one wider tensor are fine).  The calls are asynchronous, run on
- * the context's stream, allocate their workspace from its pool and can be captured into a graph, which keeps its own.
+ * each other (rows of two tensors may interleave: halves of one wider tensor are fine), which is refused with
+ * B200CONV_E_INVALID before anything runs.  The calls are asynchronous, run on the context's stream, allocate their
+ * workspace from its pool and can be captured into a graph, which keeps its own.
  * Results do not depend on timing: every sum has a fixed order. */
 typedef struct b200conv_rows {
   int64_t row, seq;
@@ -242,11 +243,12 @@ typedef struct b200conv_rows {
 
 /* Layer norm over the C channels of sequences * length rows.
  *   t = x + residual (rounded to the tensors' type), y = (t - mean) * rstd * gamma + beta, rstd = 1 / sqrt(var + eps)
- * residual, gamma, beta, total and stats may be NULL.  total receives t (it may be x or residual; y may be x too), stats
+ * residual, gamma, beta, total and stats may be NULL.  total receives t (it may be x or residual; so may y), stats
  * (mean, rstd) per row as float32 pairs.  gamma and beta hold C values of the tensors' type, or float32 with param_f32.
  * The gradient takes t as x, and stats as the forward call left them:
  *   dx = rstd * (g - mean(g) - hat * mean(g * hat)) + dtotal, g = dy * gamma, hat = (x - mean) * rstd
- * dx may be dy or dtotal; dtotal (the gradient that reaches t on other ways), dgamma and dbeta may be NULL. */
+ * dx may be dy, x or dtotal, dgamma or dbeta may be gamma; dtotal (the gradient that reaches t on other ways), dgamma and
+ * dbeta may be NULL. */
 typedef struct b200conv_norm_desc {
   int64_t sequences, length;
   int32_t C, dtype, param_f32;
@@ -267,8 +269,9 @@ int b200conv_layer_norm_grad(b200conv_ctx* ctx, const b200conv_norm_desc* d, con
  * Packed sequences (`packed`): the tensors have `length` rows, sequence i takes rows starts[i] to starts[i + 1] - 1, with
  * sequences + 1 offsets in device memory that do not decrease and do not exceed length; sequences may be empty, rows of no
  * sequence are neither read nor written.  Offsets that break this give wrong results, no access outside of the tensors.
- * The gradient: dx, and where given dw and dbias (like w, bias) and dinitial (like initial, may be it).
- * The step takes one token of every sequence ([sequences][C]: length 1) and moves `state`, like initial, on in place. */
+ * The gradient: dx, and where given dw and dbias (like w, bias; they may be those) and dinitial (like initial, may be it).  y and dx are
+ * none of the inputs: a run of tokens reads the ones before it, which another block writes.
+ * The step takes one token of every sequence ([sequences][C]: length 1) and moves `state`, like initial, on in place; y may be x. */
 typedef struct b200conv_causal_desc {
   int64_t sequences, length;
   int32_t C, width, dtype, param_f32, flip, silu, packed, reserved;
@@ -289,10 +292,11 @@ int b200conv_causal_conv_step(b200conv_ctx* ctx, const b200conv_causal_desc* d, 
  * for channels c of group g = c / (C / groups).  x, dt, z, y have C channels, B and C rows of groups * N elements; A [C][N], D and
  * dt_bias [C] are float32; D, z and dt_bias may be NULL.  A is at most 0 and delta at least 0 in such layers; results follow the formulas
  * elsewhere too, as far as float32 reaches.  1 <= N <= 128.  initial and final: float32 states [sequences][C][N] before the
- * first (NULL: zeros) and behind the last token; they may be one array.  Packed sequences as above; `longest` is an upper bound of their
+ * first (NULL: zeros) and behind the last token; they may be one array, and y may be x, dt or z.  Packed sequences as above; `longest` is an upper bound of their
  * lengths that only guides the cut of the work (0: not known).
  * The gradient takes the forward call's inputs, dy and, where given, dfinal (like final), and writes dx, ddt, dA, dB, dC, dz (with z), and
- * where given dD, ddt_bias and dinitial (like initial, may be it or dfinal); rows of no sequence are left as they were.  Its workspace is the
+ * where given dD, ddt_bias and dinitial (like initial); rows of no sequence are left as they were.  dx, ddt and dz may be dy, x, dt or z,
+ * dB and dC B or C, dA A, dD and ddt_bias D or dt_bias, dinitial initial or dfinal.  Its workspace is the
  * float32 states of every channel for each fourth token and, for every 2048 / N' channels of a group (N': N rounded up to 16, 32, 64 or
  * 128), one pair of float32 B and C rows per token.  It multiplies the decays of stretches of tokens: where growing ones exceed float32
  * together, gradients before and behind them may be infinite or NaN although their own sums would not be.

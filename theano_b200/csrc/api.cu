@@ -18,6 +18,7 @@
 #include <vector>
 
 #include "internal.h"
+#include "overlap.h"
 #include "sequence.h"
 #include "staging.h"
 
@@ -3394,6 +3395,22 @@ static int check_rows(b200conv_ctx* c, const char* name, const void* p, const b2
                 (long long)r.row, (long long)r.seq);
   return 0;
 }
+// Results overlap neither inputs nor each other, but where an input may be replaced by a result of its place and strides (`in_place`, by the
+// inputs' order) or the call keeps a copy (`any`).
+static int check_memory(b200conv_ctx* c, std::initializer_list<Region> results, std::initializer_list<Region> inputs) {
+  for (const Region* r = results.begin(); r != results.end(); ++r) {
+    if (r->empty()) continue;
+    if (folded(*r)) return fail(c, B200CONV_E_INVALID, "%s: rows overlap each other", r->name);
+    for (const Region* o = results.begin(); o != r; ++o)
+      if (overlap(*r, *o)) return fail(c, B200CONV_E_INVALID, "%s overlaps %s: two results in the same memory", r->name, o->name);
+    unsigned bit = 1;
+    for (const Region* i = inputs.begin(); i != inputs.end(); ++i, bit <<= 1)
+      if (!(r->any & bit) && overlap(*r, *i) && !((r->in_place & bit) && same_place(*r, *i)))
+        return fail(c, B200CONV_E_INVALID, r->in_place & bit ? "%s overlaps %s: it may replace it in its place, with its strides" : "%s overlaps %s, which the call reads",
+                    r->name, i->name);
+  }
+  return 0;
+}
 static int check_sizes(b200conv_ctx* c, long long sequences, long long length, long long C, int dtype) {
   if (dtype != B200CONV_F32 && dtype != B200CONV_F16 && dtype != B200CONV_BF16)
     return fail(c, B200CONV_E_INVALID, "dtype must be float32, float16 or bfloat16");
@@ -3420,6 +3437,14 @@ int b200conv_layer_norm(b200conv_ctx* c, const b200conv_norm_desc* d, const void
       (rc = check_rows(c, "y", y, d->y, d->sequences, d->length, d->C, d->dtype, true)) || (rc = check_rows(c, "total", total, d->total, d->sequences, d->length, d->C, d->dtype, true)))
     return rc;
   if ((rc = check_aligned(c, {gamma, beta}, d->param_f32 ? 4 : row_elem_size(d->dtype))) || (rc = check_aligned(c, {stats}, 8))) return rc;
+  const size_t es = row_elem_size(d->dtype), pbytes = (d->param_f32 ? 4 : es) * d->C;
+  auto rows = [&](const char* name, const void* p, const b200conv_rows& r, int width, unsigned in_place = 0) {
+    return region(name, p, r, d->sequences, d->length, width, es, in_place);
+  };
+  if ((rc = check_memory(c, {rows("y", y, d->y, std::max(d->C, d->y.stored), 3), rows("total", total, d->total, std::max(d->C, d->total.stored), 3),
+                             region("stats", stats, 8 * static_cast<size_t>(d->sequences * d->length))},
+                         {rows("x", x, d->x, d->C), rows("the residual", residual, d->residual, d->C), region("gamma", gamma, pbytes), region("beta", beta, pbytes)})))
+    return rc;
   NormArgs a = {};
   a.d = *d;
   a.x = x; a.residual = residual; a.gamma = gamma; a.beta = beta; a.y = y; a.total = total; a.stats = stats;
@@ -3447,6 +3472,13 @@ int b200conv_layer_norm_grad(b200conv_ctx* c, const b200conv_norm_desc* d, const
       (rc = check_rows(c, "dtotal", dtotal, d->dtotal, d->sequences, d->length, d->C, d->dtype)) || (rc = check_rows(c, "dx", dx, d->dx, d->sequences, d->length, d->C, d->dtype, true)))
     return rc;
   if ((rc = check_aligned(c, {gamma, dgamma, dbeta}, d->param_f32 ? 4 : row_elem_size(d->dtype))) || (rc = check_aligned(c, {stats}, 8))) return rc;
+  auto rows = [&](const char* name, const void* p, const b200conv_rows& r, int width, unsigned in_place = 0) {
+    return region(name, p, r, d->sequences, d->length, width, row_elem_size(d->dtype), in_place);
+  };
+  if ((rc = check_memory(c, {rows("dx", dx, d->dx, std::max(d->C, d->dx.stored), 7), region("dgamma", dgamma, pbytes, 8), region("dbeta", dbeta, pbytes, 8)},
+                         {rows("dy", dy, d->dy, d->C), rows("x", x, d->x, d->C), rows("dtotal", dtotal, d->dtotal, d->C), region("gamma", gamma, pbytes),
+                          region("stats", stats, 8 * static_cast<size_t>(d->sequences * d->length))})))
+    return rc;
   Scratch tmp(c);
   NormArgs a = {};
   a.d = *d;
@@ -3496,6 +3528,13 @@ static int check_causal(b200conv_ctx* c, const b200conv_causal_desc* d, const vo
 static size_t causal_state_bytes(const b200conv_causal_desc* d) {
   return row_elem_size(d->dtype) * static_cast<size_t>(d->sequences) * (d->width - 1) * d->C;
 }
+// A parameter of n values per channel, offsets of packed sequences.
+static Region param_region(const b200conv_causal_desc* d, const char* name, const void* p, int n, unsigned in_place = 0) {
+  return region(name, p, (d->param_f32 ? 4 : row_elem_size(d->dtype)) * static_cast<size_t>(d->C) * n, in_place);
+}
+static Region starts_region(int packed, long long sequences, const int32_t* starts) {
+  return region("the offsets", packed ? starts : nullptr, sizeof(int32_t) * static_cast<size_t>(sequences + 1));
+}
 
 int b200conv_causal_conv(b200conv_ctx* c, const b200conv_causal_desc* d, const void* x, const void* w, const void* bias, const void* initial,
                          const int32_t* starts, void* y, void* final) {
@@ -3507,11 +3546,17 @@ int b200conv_causal_conv(b200conv_ctx* c, const b200conv_causal_desc* d, const v
   if (!d->C || !d->sequences) return 0;
   if (d->length && !y) return fail(c, B200CONV_E_INVALID, "causal convolution without output");
   if (!d->length && !final) return 0;
+  const size_t es = row_elem_size(d->dtype), state = causal_state_bytes(d);
+  const long long n = d->packed ? 1 : d->sequences;
+  if ((rc = check_memory(c, {region("y", y, d->y, n, d->length, std::max(d->C, d->y.stored), es), region("final", final, state, 0, 8)},
+                         {region("x", x, d->x, n, d->length, d->C, es), param_region(d, "w", w, d->width), param_region(d, "bias", bias, 1),
+                          region("initial", initial, state), starts_region(d->packed, d->sequences, starts)})))
+    return rc;
   Scratch tmp(c);
   CausalArgs a = {};
   a.d = *d;
   a.x = x; a.w = w; a.bias = bias; a.initial = initial; a.starts = d->packed ? starts : nullptr; a.y = y; a.final = final;
-  if ((rc = detach_state(c, tmp, &a.initial, final, causal_state_bytes(d)))) return rc;
+  if ((rc = detach_state(c, tmp, &a.initial, final, state))) return rc;
   KLAUNCH(c, kKCausal, launch_causal_conv(a, c->stream));
   return 0;
 }
@@ -3534,12 +3579,18 @@ int b200conv_causal_conv_grad(b200conv_ctx* c, const b200conv_causal_desc* d, co
     return 0;
   }
   if (!dy || !dx) return fail(c, B200CONV_E_INVALID, "causal convolution gradient without dy or dx");
+  const size_t es = row_elem_size(d->dtype), state = causal_state_bytes(d);
+  if ((rc = check_memory(c, {region("dx", dx, d->dx, n, d->length, std::max(d->C, d->dx.stored), es), param_region(d, "dw", dw, d->width, 4),
+                             param_region(d, "dbias", dbias, 1, 8), region("dinitial", dinitial, state, 0, 16)},
+                         {region("dy", dy, d->dy, n, d->length, d->C, es), region("x", x, d->x, n, d->length, d->C, es), param_region(d, "w", w, d->width),
+                          param_region(d, "bias", bias, 1), region("initial", initial, state), starts_region(d->packed, d->sequences, starts)})))
+    return rc;
   Scratch tmp(c);
   CausalArgs a = {};
   a.d = *d;
   a.dy = dy; a.x = x; a.w = w; a.bias = bias; a.initial = initial; a.starts = d->packed ? starts : nullptr;
   a.dx = dx; a.dw = dw; a.dbias = dbias; a.dinitial = dinitial;
-  if ((rc = detach_state(c, tmp, &a.initial, dinitial, causal_state_bytes(d)))) return rc;
+  if ((rc = detach_state(c, tmp, &a.initial, dinitial, state))) return rc;
   if ((dw || dbias) && (rc = tmp.get(sizeof(float) * (d->width + 1) * d->C * static_cast<size_t>(causal_grad_parts(a)),
                                      reinterpret_cast<void**>(&a.partial))))
     return rc;
@@ -3558,6 +3609,10 @@ int b200conv_causal_conv_step(b200conv_ctx* c, const b200conv_causal_desc* d, co
   if (rc || (rc = check_rows(c, "y", y, d->y, d->sequences, 1, d->C, d->dtype, true))) return rc;
   if (!d->C || !d->sequences) return 0;
   if (!state || !y) return fail(c, B200CONV_E_INVALID, "causal convolution step without state or output");
+  const size_t es = row_elem_size(d->dtype);
+  if ((rc = check_memory(c, {region("y", y, d->y, d->sequences, 1, std::max(d->C, d->y.stored), es, 1), region("state", state, causal_state_bytes(d))},
+                         {region("x", x, d->x, d->sequences, 1, d->C, es), param_region(d, "w", w, d->width), param_region(d, "bias", bias, 1)})))
+    return rc;
   CausalArgs a = {};
   a.d = *d;
   a.x = x; a.w = w; a.bias = bias; a.final = state; a.y = y;
@@ -3589,6 +3644,20 @@ static int check_scan(b200conv_ctx* c, const b200conv_scan_desc* d, const void* 
   return check_rows(c, "C", C, d->Cm, n, d->length, gn, d->dtype);
 }
 
+// The memory of a scan's tensors.
+struct ScanRegions {
+  const b200conv_scan_desc* d;
+  long long n;
+  size_t es;
+  explicit ScanRegions(const b200conv_scan_desc* desc) : d(desc), n(desc->packed ? 1 : desc->sequences), es(row_elem_size(desc->dtype)) {}
+  Region channels(const char* name, const void* p, const b200conv_rows& r, unsigned in_place = 0) const { return region(name, p, r, n, d->length, d->C, es, in_place); }
+  Region states(const char* name, const void* p, const b200conv_rows& r, unsigned in_place = 0) const {
+    return region(name, p, r, n, d->length, 1LL * d->groups * d->N, es, in_place);
+  }
+  Region matrix(const char* name, const void* p, unsigned in_place = 0) const { return region(name, p, sizeof(float) * d->C * d->N, in_place); }
+  Region vector(const char* name, const void* p, unsigned in_place = 0) const { return region(name, p, sizeof(float) * d->C, in_place); }
+};
+
 int b200conv_selective_scan(b200conv_ctx* c, const b200conv_scan_desc* d, const void* x, const void* dt, const float* A, const void* B, const void* C,
                             const float* D, const void* z, const float* dt_bias, const float* initial, const int32_t* starts, void* y, float* final) {
   if (!c) return B200CONV_E_INVALID;
@@ -3605,6 +3674,12 @@ int b200conv_selective_scan(b200conv_ctx* c, const b200conv_scan_desc* d, const 
     else CU_OK(c, cudaMemsetAsync(final, 0, state_bytes, c->stream));
     return 0;
   }
+  const ScanRegions in(d);
+  // every lane reads a token's x, dt and z before it writes y there, and no other lane's
+  if ((rc = check_memory(c, {in.channels("y", y, d->y, 7), region("final", final, state_bytes, 0, 1u << 8)},
+                         {in.channels("x", x, d->x), in.channels("dt", dt, d->dt), in.channels("z", z, d->z), in.matrix("A", A), in.states("B", B, d->B),
+                          in.states("C", C, d->Cm), in.vector("D", D), in.vector("dt_bias", dt_bias), region("initial", initial, state_bytes), starts_region(d->packed, d->sequences, starts)})))
+    return rc;
   Scratch tmp(c);
   ScanArgs a = {};
   a.d = *d;
@@ -3660,6 +3735,15 @@ int b200conv_selective_scan_grad(b200conv_ctx* c, const b200conv_scan_desc* d, c
     return 0;
   }
   if (!dy || !dx || !ddt || !dB || !dC || (z && !dz)) return fail(c, B200CONV_E_INVALID, "selective scan gradient without dy, dx, ddt, dB, dC or dz");
+  const ScanRegions in(d);
+  // dx, ddt and dz are written where a block has taken dy, x, dt and z from, the sums over blocks by kernels behind the last that reads B, C, A, D and the bias
+  if ((rc = check_memory(c, {in.channels("dx", dx, d->dx, 15), in.channels("ddt", ddt, d->ddt, 15), in.channels("dz", dz, d->dz, 15), in.states("dB", dB, d->dB, 96),
+                             in.states("dC", dC, d->dCm, 96), in.matrix("dA", dA, 16), in.vector("dD", dD, 384), in.vector("ddt_bias", ddt_bias, 384),
+                             region("dinitial", dinitial, state_bytes, 0, 1536)},
+                         {in.channels("dy", dy, d->dy), in.channels("x", x, d->x), in.channels("dt", dt, d->dt), in.channels("z", z, d->z), in.matrix("A", A),
+                          in.states("B", B, d->B), in.states("C", C, d->Cm), in.vector("D", D), in.vector("dt_bias", dt_bias),
+                          region("initial", initial, state_bytes), region("dfinal", dfinal, state_bytes), starts_region(d->packed, d->sequences, starts)})))
+    return rc;
   Scratch tmp(c);
   ScanArgs a = {};
   a.d = *d;
@@ -3696,6 +3780,11 @@ int b200conv_selective_scan_step(b200conv_ctx* c, const b200conv_scan_desc* d, c
   if (rc || (rc = check_rows(c, "y", y, d->y, d->sequences, 1, d->C, d->dtype, true))) return rc;
   if (!d->C || !d->sequences) return 0;
   if (!state || !y) return fail(c, B200CONV_E_INVALID, "selective scan step without state or output");
+  const ScanRegions in(d);
+  if ((rc = check_memory(c, {in.channels("y", y, d->y, 7), region("state", state, sizeof(float) * static_cast<size_t>(d->sequences) * d->C * d->N)},
+                         {in.channels("x", x, d->x), in.channels("dt", dt, d->dt), in.channels("z", z, d->z), in.matrix("A", A), in.states("B", B, d->B),
+                          in.states("C", C, d->Cm), in.vector("D", D), in.vector("dt_bias", dt_bias)})))
+    return rc;
   ScanArgs a = {};
   a.d = *d;
   a.x = x; a.dt = dt; a.A = A; a.B = B; a.C = C; a.D = D; a.z = z; a.dt_bias = dt_bias; a.final = state; a.y = y;

@@ -4,7 +4,8 @@ Beside the convolutions of ``theano_b200.shim`` and in the same two forms: numpy
 ``perform`` calls) and ``device_*`` calls on tensors that stay in HBM, which are asynchronous on their context's stream.
 Sequence tensors are ``(sequences, tokens, channels)`` with contiguous channels; sequences of several lengths may lie one
 behind the other in a ``(rows, channels)`` tensor (`Sequences`).  A channels-last ``shim.DeviceTensor`` counts as one with
-its pixels as tokens.  Data types: float32, float16 and bfloat16; sums and states are float32.
+its pixels as tokens.  Data types: float32, float16 and bfloat16; sums and states are float32.  A result's memory is that of an input
+only where a call says so; other overlaps raise ValueError.
 
 The reference runs causal convolutions through its 2-D convolution (theano/tensor/nnet/abstract_conv.py, causal_conv1d) and
 recurrences through its scan op, one op call per token; nothing here computes on the CPU.
@@ -313,7 +314,7 @@ def device_layer_norm(x, gamma=None, beta=None, eps=1e-5, residual=None, total=N
 
     `gamma`, `beta`: vectors of the tensors' type or float32.  `residual`: added to x first; `total` receives the sum,
     rounded to the tensors' type, which is what is normalised (it may be x or residual themselves).  `stats`: float32 of
-    x's shape with (mean, rstd) in place of the channels, for the gradient.  Returns `out` (which may be x)."""
+    x's shape with (mean, rstd) in place of the channels, for the gradient.  Returns `out` (which may be x or residual, not `total`)."""
     given, x = x, _array(x)
     ctx = x.ctx
     gamma, beta, residual, total, stats = _array(gamma), _array(beta), _array(residual), _array(total), _array(stats)
@@ -332,7 +333,7 @@ def device_layer_norm(x, gamma=None, beta=None, eps=1e-5, residual=None, total=N
 def device_layer_norm_grad(dy, x, gamma, stats, dtotal=None, out=None, dgamma=None, dbeta=None):
     """Gradients (dx, dgamma, dbeta) of `device_layer_norm`; x is what was normalised (`total` where there was a
     residual) and `stats` what the forward call left.  `dtotal`, the gradient that reaches the sum on other ways, is added to
-    dx, which may be dy or dtotal.  dgamma and dbeta have gamma's type (float32 without one); False leaves one out."""
+    dx, which may be dy, x or dtotal.  dgamma and dbeta have gamma's type (float32 without one); False leaves one out."""
     given, dy = dy, _array(dy)
     ctx = dy.ctx
     x, gamma, stats, dtotal = _array(x), _array(gamma), _array(stats), _array(dtotal)
@@ -426,7 +427,7 @@ def device_causal_conv1d(x, w, bias=None, silu=False, filter_flip=True, initial=
 
     `w`: (channels, taps), 2 to 8 taps; `initial`: (sequences, taps - 1, channels), the tokens before the first, oldest
     first (default: zeros); `final` receives the same behind the last token and may be `initial`.  With `sequences`
-    x is (rows, channels).  Returns `out`."""
+    x is (rows, channels).  Returns `out`, which is none of the inputs."""
     given, x, w, bias = x, _array(x), _array(w), _array(bias)
     ctx = x.ctx
     initial, final = _array(initial), _array(final)
@@ -446,7 +447,8 @@ def device_causal_conv1d(x, w, bias=None, silu=False, filter_flip=True, initial=
 def device_causal_conv1d_grad(dy, x, w, bias=None, silu=False, filter_flip=True, initial=None, sequences=None, out=None, dw=None, dbias=None,
                               dinitial=None):
     """Gradients (dx, dw, dbias, dinitial) of `device_causal_conv1d`.  dw and dbias have the types of w and bias (False
-    leaves one out, dbias exists with a bias only), dinitial is computed where it is given."""
+    leaves one out, dbias exists with a bias only), dinitial is computed where it is given and may be `initial`.  dx is none of the
+    inputs."""
     given, dy, x, w, bias = dy, _array(dy), _array(x), _array(w), _array(bias)
     ctx = x.ctx
     initial, dinitial = _array(initial), _array(dinitial)
@@ -564,7 +566,7 @@ def device_selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus
 
     x, dt, z: (sequences, tokens, channels), or (rows, channels) with `sequences`; B, C: the same rows of (groups, states) or
     (states,), shared by the channels of a group; A (channels, states), D and dt_bias (channels,) float32.  `initial` and `final`:
-    float32 (sequences, channels, states), which may be one array.  Returns `out`, which is none of the inputs."""
+    float32 (sequences, channels, states), which may be one array.  Returns `out`, which may be x, dt or z."""
     given, x, dt, A, B, C = x, _array(x), _array(dt), _array(A), _array(B), _array(C)
     ctx = x.ctx
     D, z, dt_bias, initial, final = _array(D), _array(z), _array(dt_bias), _array(initial), _array(final)
@@ -613,7 +615,8 @@ def device_selective_scan_grad(dy, x, dt, A, B, C, D=None, z=None, dt_bias=None,
                                grads=None):
     """Gradients of `device_selective_scan` for dy and, where given, `dfinal`, the gradient of the final states: a dict with
     x, dt, A, B, C and, where the call has them, D, z, dt_bias and initial.  `grads`: tensors to write them into, of the inputs'
-    shapes and types; those that it lacks are made."""
+    shapes and types, which may be the inputs themselves (that of x, dt and z also dy, that of initial also dfinal); those that it
+    lacks are made."""
     dy, x, dt, A, B, C = _array(dy), _array(x), _array(dt), _array(A), _array(B), _array(C)
     ctx = x.ctx
     D, z, dt_bias, initial, dfinal = _array(D), _array(z), _array(dt_bias), _array(initial), _array(dfinal)
