@@ -25,6 +25,7 @@ _CODES = {np.dtype(np.float32): F32, np.dtype(np.float16): F16, BFLOAT16: BF16}
 _DTYPES = {F32: np.dtype(np.float32), F16: np.dtype(np.float16), BF16: BFLOAT16}
 _INT32 = np.dtype(np.int32)
 _OTHER = -1                              # code of tensors that are no operands (offsets)
+_FREED = "the memory of this tensor has been freed"
 
 
 _signatures = {}                         # what plans need to know of an array -> a number that stands for it
@@ -99,7 +100,13 @@ class DeviceArray(object):
         """Elements from the first to behind the last one."""
         return 1 + sum((n - 1) * s for n, s in zip(self.shape, self.strides)) if self.size else 0
 
+    @property
+    def freed(self):
+        return self.ptr is None or (self._base is not None and self._base.ptr is None)
+
     def __getitem__(self, key):
+        if self.freed:
+            raise ValueError(_FREED)
         key = key if isinstance(key, tuple) else (key,)
         if len(key) > len(self.shape) or any(k is Ellipsis or k is None for k in key):
             raise IndexError("too many indices, or neither integers nor slices")
@@ -119,16 +126,19 @@ class DeviceArray(object):
                     raise IndexError("index %d of axis %d (extent %d; the last axis takes slices)" % (k, axis, n))
                 at += (k % n) * self.strides[axis]
         whole = shape[-1] == self.shape[-1]
-        return DeviceArray(self.ctx, shape, self.dtype, strides, (self.ptr or 0) + at * self.dtype.itemsize, self.stored if whole else 0, self)
+        return _View(self.ctx, shape, self.dtype, strides, self.ptr + at * self.dtype.itemsize, self.stored if whole else 0,
+                     self if self._base is None else self._base)
 
-    @classmethod
-    def rows_of(cls, image):
+    @staticmethod
+    def rows_of(image):
         """The (N, H * W, C) rows of a channels-last `shim.DeviceTensor`."""
         if image.layout != "nhwc":
             raise ValueError("sequence operators take channels-last tensors")
+        if image.ptr is None:
+            raise ValueError(_FREED)
         n, c, h, w = image.shape
         cp = image.stored_channels
-        return cls(image.ctx, (n, h * w, c), image.dtype, (h * w * cp, cp, 1), image.ptr, cp, image)
+        return _View(image.ctx, (n, h * w, c), image.dtype, (h * w * cp, cp, 1), image.ptr, cp, image)
 
     @classmethod
     def from_host(cls, ctx, arr, dtype=None):
@@ -144,6 +154,8 @@ class DeviceArray(object):
 
     def to_host(self):
         """A numpy array of the values (bfloat16: as float32)."""
+        if self.freed:
+            raise ValueError(_FREED)
         flat = np.empty(self.span, self.dtype)
         self.ctx.d2h(flat, self.ptr)
         self.ctx.sync()
@@ -165,6 +177,10 @@ class DeviceArray(object):
                 self.free()
         except Exception:
             pass
+
+
+class _View(DeviceArray):
+    """Memory of another tensor: checked on every use, since that one may be freed before its views are gone."""
 
 
 class Sequences(object):
@@ -220,9 +236,13 @@ def _array(t):
     if isinstance(t, DeviceTensor):
         if t.layout == "nhwc":
             return DeviceArray.rows_of(t)
+        if t.ptr is None:
+            raise ValueError(_FREED)
         n = t.shape[0] * t.shape[1] * t.shape[2] * t.shape[3]
         return DeviceArray(t.ctx, (n,), t.dtype, (1,), t.ptr, 0, t)
     if isinstance(t, DeviceArray):
+        if t.freed:
+            raise ValueError(_FREED)
         return t
     raise TypeError("expected a DeviceArray or a channels-last DeviceTensor, not %s" % type(t).__name__)
 
@@ -232,7 +252,12 @@ def _sig(t):
 
 
 def _ptr(t):
-    return None if t is None else t.ptr
+    """Of an argument that may be left out; one that was freed is not (for the others the library refuses a null pointer)."""
+    if t is None:
+        return None
+    if t.ptr is None:
+        raise ValueError(_FREED)
+    return t.ptr
 
 
 def _one_context(ctx, *tensors):
