@@ -70,3 +70,23 @@ def test_wrapped_memory_and_empty_tensors_are_not_freed_ones(ctx):
     empty = Q.DeviceArray(ctx, (0, 9, 8), np.float32, (72, 8, 1), _ptr=0)
     Q.device_layer_norm(empty, out=Q.DeviceArray(ctx, (0, 9, 8), np.float32))
     assert len(ctx.lib.calls) == 2
+
+
+def test_pad_channels_of_a_scans_inputs(ctx):
+    """Inputs may be images with pad channels; results, whose pad channels a scan does not write, may not: in steps neither."""
+    padded = lambda: Q.DeviceArray(ctx, (2, 9, 6), np.float32, (72, 8, 1), 1 << 20, 8)  # noqa: E731
+    A, bc = arr(ctx, 6, 4), lambda: arr(ctx, 2, 9, 4)  # noqa: E731
+    Q.device_selective_scan(padded(), padded(), A, bc(), bc(), z=padded(), out=arr(ctx, 2, 9, 6))
+    own = dict(x=arr(ctx, 2, 9, 6), dt=arr(ctx, 2, 9, 6), z=arr(ctx, 2, 9, 6))
+    Q.device_selective_scan_grad(padded(), padded(), padded(), A, bc(), bc(), z=padded(), grads=own)
+    token, states, b = padded()[:, 0], arr(ctx, 2, 6, 4), arr(ctx, 2, 4)
+    Q.device_selective_scan_step(token, token, A, b, b, states, z=token, out=arr(ctx, 2, 6))
+    assert len(ctx.lib.calls) == 3
+    for call in (lambda: Q.device_selective_scan(padded(), padded(), A, bc(), bc(), out=padded()),
+                 lambda: Q.device_selective_scan_grad(padded(), padded(), padded(), A, bc(), bc(), z=padded(), grads=dict(own, dt=padded())),
+                 lambda: Q.device_selective_scan_grad(padded(), padded(), padded(), A, bc(), bc(), z=padded(), grads=dict(own, z=padded())),
+                 lambda: Q.device_selective_scan_grad(padded(), padded(), padded(), A, bc(), bc(), grads=dict(x=padded())),
+                 lambda: Q.device_selective_scan_step(token, token, A, b, b, states, out=padded()[:, 1])):
+        with pytest.raises(ValueError, match="pad channels"):
+            call()
+    assert len(ctx.lib.calls) == 3

@@ -558,7 +558,7 @@ def _plan_scan(x, A, vectors, softplus, sequences, states, tensors, grouped):
     d.x = _rows(x)
     for name, t in tensors:
         _same(name, t, x.shape, code)
-        if t is not None and t.stored > C:
+        if t is not None and t.stored > C and name in ("y", "dx", "ddt", "dz"):
             raise ValueError("a selective scan writes no pad channels: %d channels are stored as %d" % (C, t.stored))
         setattr(d, name, _rows(t))
     shape = None
@@ -626,7 +626,7 @@ def device_selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=No
             raise ValueError("a step takes (sequences, channels), not %s" % (x.shape,))
 
         def token(t):                    # one token per sequence: the sequences' stride is that of the rows
-            return None if t is None else DeviceArray(t.ctx, (t.shape[0], 1) + t.shape[1:], t.dtype, (t.strides[0], t.strides[0]) + t.strides[1:], t.ptr, 0, t)
+            return None if t is None else DeviceArray(t.ctx, (t.shape[0], 1) + t.shape[1:], t.dtype, (t.strides[0], t.strides[0]) + t.strides[1:], t.ptr, t.stored, t)
         return _plan_scan(token(x), A, (("D", D), ("dt_bias", dt_bias)), softplus, None, (("state", state),),
                           (("dt", token(dt)), ("z", token(z)), ("y", token(y))), (("B", token(B)), ("Cm", token(C))))
     d = _plan(("scan step", softplus, x.sig, dt.sig, A.sig, B.sig, C.sig, state.sig, _sig(D), _sig(z), _sig(dt_bias), y.sig), make)
