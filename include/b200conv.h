@@ -350,8 +350,9 @@ int b200conv_nhwc_to_nchw(b200conv_ctx* ctx, const void* src, void* dst, int N, 
  * pooling, layout conversion, all-reduce) can be recorded once between graph_begin and graph_end
  * and replayed with one launch.  Run the sequence once before capturing it (kernel attributes
  * and the memory pool are then warm); the pointers and shapes are frozen into the graph; the
- * temporaries the calls used stay reserved until graph_destroy.  Host-pointer calls, sync,
- * timer_stop and barrier are refused while a capture is open. */
+ * temporaries the calls used stay reserved until graph_destroy, and so do blocks of b200conv_malloc that are freed while a
+ * capture is open, or later if they were made in it.  Other blocks that a graph uses must outlive it.  Host-pointer calls,
+ * sync, timer_stop and barrier are refused while a capture is open. */
 int b200conv_graph_begin(b200conv_ctx* ctx);
 int b200conv_graph_end(b200conv_ctx* ctx, b200conv_graph** graph);
 int b200conv_graph_launch(b200conv_ctx* ctx, b200conv_graph* graph);

@@ -123,6 +123,10 @@ struct b200conv_ctx {
   // pooled device memory: free blocks by size, live blocks by address
   std::multimap<size_t, void*> free_blocks;
   std::map<void*, size_t> live;
+  // memory of captured graphs: blocks that were made during a capture and are still the caller's, and blocks that the caller freed and
+  // that replays go on using (with their sizes; the same capture may hand them out again, as one replay follows the capture's order)
+  std::map<void*, b200conv_graph*> held;
+  std::map<void*, std::pair<size_t, b200conv_graph*>> parked;
   size_t pool_bytes = 0;
   void* l2buf = nullptr;
   size_t l2bytes = 0;
@@ -247,6 +251,14 @@ struct DeviceGuard {
 int pool_alloc(b200conv_ctx* c, size_t bytes, void** out) {
   if (bytes == 0) bytes = 256;
   bytes = (bytes + 255) & ~static_cast<size_t>(255);
+  if (c->capturing)
+    for (auto k = c->parked.begin(); k != c->parked.end(); ++k)
+      if (k->second.second == c->capturing && k->second.first >= bytes && k->second.first <= bytes + bytes / 4 + (1 << 20)) {
+        *out = k->first;
+        c->live[*out] = k->second.first;
+        c->parked.erase(k);
+        return 0;
+      }
   auto it = c->free_blocks.lower_bound(bytes);
   if (it != c->free_blocks.end() && it->first <= bytes + bytes / 4 + (1 << 20)) {
     *out = it->second;
@@ -288,6 +300,17 @@ int pool_free(b200conv_ctx* c, void* p) {
 }
 
 // Temporaries of one call: returned to the pool when the call ends.
+// What a graph kept goes back to the pool; blocks that are still the caller's are his alone.
+void release_graph(b200conv_ctx* c, b200conv_graph* gr) {
+  for (void* p : gr->retained) pool_free(c, p);
+  for (auto k = c->held.begin(); k != c->held.end();) k = k->second == gr ? c->held.erase(k) : std::next(k);
+  for (auto k = c->parked.begin(); k != c->parked.end();) {
+    if (k->second.second != gr) { ++k; continue; }
+    c->free_blocks.insert({k->second.first, k->first});
+    k = c->parked.erase(k);
+  }
+}
+
 struct Scratch {
   b200conv_ctx* c;
   std::vector<void*> ptrs;
@@ -3136,6 +3159,7 @@ void b200conv_destroy(b200conv_ctx* c) {
   b200conv_nccl_destroy(c);
   for (auto& kv : c->free_blocks) cudaFree(kv.second);
   for (auto& kv : c->live) cudaFree(kv.first);
+  for (auto& kv : c->parked) cudaFree(kv.first);
   if (c->l2buf) cudaFree(c->l2buf);
   if (c->d_token) cudaFree(c->d_token);
   if (c->up_stream) {
@@ -3798,7 +3822,9 @@ int b200conv_malloc(b200conv_ctx* c, size_t bytes, void** dptr) {
   if (!c || !dptr) return B200CONV_E_INVALID;
   std::lock_guard<std::mutex> g(c->mu);
   DeviceGuard dg(c->device);
-  return pool_alloc(c, bytes, dptr);
+  const int rc = pool_alloc(c, bytes, dptr);
+  if (rc == 0 && c->capturing) c->held[*dptr] = c->capturing;
+  return rc;
 }
 int b200conv_free(b200conv_ctx* c, void* dptr) {
   if (!c) return B200CONV_E_INVALID;
@@ -3809,6 +3835,15 @@ int b200conv_free(b200conv_ctx* c, void* dptr) {
     const char *lo = static_cast<const char*>(dptr), *hi = lo + it->second;
     for (auto& kv : c->packed)
       if (kv.second.src >= lo && kv.second.src < hi) kv.second.valid = false;
+    // freed while a graph is captured, or made for one that still exists: its replays use the block
+    auto made = c->held.find(dptr);
+    b200conv_graph* user = c->capturing ? c->capturing : made != c->held.end() ? made->second : nullptr;
+    if (made != c->held.end()) c->held.erase(made);
+    if (user) {
+      c->parked[dptr] = {it->second, user};
+      c->live.erase(it);
+      return 0;
+    }
   }
   return pool_free(c, dptr);
 }
@@ -3969,7 +4004,7 @@ int b200conv_graph_end(b200conv_ctx* c, b200conv_graph** out) {
   if (e == cudaSuccess && rc == 0) e = cudaGraphInstantiate(&gr->exec, gr->graph, 0);
   if (e != cudaSuccess || rc) {
     cudaGetLastError();
-    for (void* p : gr->retained) pool_free(c, p);
+    release_graph(c, gr);
     if (gr->graph) cudaGraphDestroy(gr->graph);
     delete gr;
     return rc ? rc : fail(c, B200CONV_E_CUDA, "graph capture failed: %s", cudaGetErrorString(e));
@@ -3995,7 +4030,7 @@ int b200conv_graph_destroy(b200conv_ctx* c, b200conv_graph* gr) {
   cudaStreamSynchronize(c->stream);
   if (gr->exec) cudaGraphExecDestroy(gr->exec);
   if (gr->graph) cudaGraphDestroy(gr->graph);
-  for (void* p : gr->retained) pool_free(c, p);
+  release_graph(c, gr);
   delete gr;
   return 0;
 }

@@ -372,7 +372,8 @@ class Context(object):
     # -- CUDA graphs -------------------------------------------------------------------------
     def capture(self, fn):
         """Run ``fn()`` (device-pointer calls only) under stream capture; returns a ``Graph``.
-        Call ``fn()`` once eagerly beforehand so that the memory pool is warm."""
+        Call ``fn()`` once eagerly beforehand so that the memory pool is warm.  Tensors that ``fn`` makes may be dropped, there or
+        later: their memory stays with the graph.  Those it takes from outside must outlive the graph."""
         self.check(self.lib.b200conv_graph_begin(self.h))
         try:
             fn()
