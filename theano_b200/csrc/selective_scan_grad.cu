@@ -12,7 +12,7 @@
 // add over the channels goes through shared memory, 32 values per lane and token.  4 x 2048 tokens, 2048 channels, 16 states, bfloat16:
 // 157 us the first, 419 the second, 17 the sums over blocks and pieces.  The second takes 385 instructions, 106 accesses to shared
 // memory (424 clocks of an SM quarter) and 36 exponentials (288) per token and warp and is bound by neither: with 250 registers two
-// blocks fit an SM, and two warps per quarter leave 60 % of the issue slots empty.  Four states to a lane with sums by shuffles took 525 us
+// blocks fit an SM (one of cut float32 sequences, whose shared memory is 118 KB), and two warps per quarter leave 60 % of the issue slots empty.  Four states to a lane with sums by shuffles took 525 us
 // at 3 blocks, eight states 567; limits of 168 registers spill 180 of them.
 #include "selective_scan.cuh"
 
@@ -541,7 +541,11 @@ __global__ void __launch_bounds__(256) scan_params_kernel(ScanArgs a) {
 int scan_grad_slots(int N) { return N <= 16 ? 16 : scan_state_slots(N); }
 long long scan_kept(const ScanArgs& a) { return a.rows / kKeep + a.pieces + 1; }
 
-// Pieces of the gradient's call.  Being cut costs three operations per state in the forward walk.
+// Pieces of the gradient's call.  Being cut costs three operations per state in the forward walk.  Counted are two blocks to an SM in every
+// form, although registers and shared memory (GradShape: 118 KB for cut float32 sequences, 118 to 130 KB over 64 states) leave cut float32
+// sequences and those of over 64 states one: the forward walk, which holds three, gains more from the finer cut than a second round of the
+// backward walk costs.  Float32, 2048 channels, 16 states, counted as two / as they fit: 9 x 2048 tokens 1844 / 2234 us, 4 x 2048 830 / 1055,
+// 1 x 8192 843 / 944; 16 x 1000 of 2560 channels 1870 / 1853; 4 x 1024 of 1024 channels and 128 states, bfloat16, 3074 / 3080.
 void plan_grad_pieces(ScanArgs* a) {
   const int wide = kScanThreads * 16 / scan_grad_slots(a->d.N), per = a->d.C / a->d.groups;
   const long long tiles = 1LL * a->d.groups * ((per + wide - 1) / wide);
