@@ -363,10 +363,12 @@ def _plain_scan_step(st):
 
 # ---- the framework's calls -----------------------------------------------------------------------------------------
 def _tensors(st):
-    """The framework's tensors over the state's memory, made once, as a program that keeps its buffers does."""
+    """The framework's tensors over the state's memory, made once, as a program that keeps its buffers does.  Who reads the results with
+    torch waits for the device first."""
     if "tensors" not in st:
         from theano_b200 import sequence, shim
         ctx = shim.get_context(0)
+        torch.cuda.synchronize()               # the inputs come from torch's stream, the calls run on the context's
 
         def wrap(t):
             return sequence.DeviceArray(ctx, t.shape, NAMES[t.dtype], strides=t.stride(), _ptr=t.data_ptr())
