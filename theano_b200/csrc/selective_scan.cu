@@ -6,7 +6,7 @@
 // sequence is cut into pieces: 16 per clock and SM, 4.6e12 a second at 1.965 GHz, which bounds prompts (at N = 16 the tensors' 8
 // bytes per token and channel take a third of that time).  So a lane holds all states of a channel, which makes everything else a
 // token costs (its loads, softplus, gate) as cheap per state as it gets, two states go through the polynomial instead of the special
-// function unit, and the rest runs on packed pairs.  8192 tokens, 2048 channels, 16 states, bfloat16: 191 us in 37 pieces.
+// function unit, and the rest runs on packed pairs.  8192 tokens, 2048 channels, 16 states, bfloat16: 181 us in 37 pieces.
 #include "selective_scan.cuh"
 
 #include <algorithm>
@@ -18,8 +18,9 @@ namespace {
 // is shared by all of them; the rows of B and C, the same for all lanes, come from shared memory as float32.
 constexpr int kScanBlocks = 4;                   // of an SM: 16 warps, 128 registers a thread
 
-// ASYNC: x, dt and z of 16-bit tensors on their boundaries come by asynchronous copies, a tile ahead, in 16 bytes (182 us, by loads
-// of two bytes per lane 190: no addresses per token, no registers for tokens on their way).
+// ASYNC: x, dt and z of 16-bit tensors on their boundaries come by asynchronous copies, a tile ahead, in 16 bytes (181 us, by loads
+// of two bytes per lane 190: no addresses per token, no registers for tokens on their way).  Float32 tiles of 16 tokens would take 52 KB
+// of shared memory, more than the 48 KB that a kernel may declare; they come by loads of four bytes.
 template <typename T, int S, int P, bool WIDE, bool LOCAL, bool ASYNC>
 __global__ void __launch_bounds__(kScanThreads, S * P <= 32 ? kScanBlocks : 1) scan_lane_kernel(ScanArgs a) {
   constexpr int NS = S * P, kWide = kScanThreads / P, kTokens = ASYNC && NS <= 32 ? 16 : tile_tokens(NS);

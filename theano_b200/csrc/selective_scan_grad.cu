@@ -10,10 +10,10 @@
 // zero states and of a zero adjoint).  The second walks backward: for four tokens at a time it makes their states again, in registers, and
 // runs the adjoint over them.  Both have a lane per channel with its states, so that sums over the states cost nothing; what dB and dC
 // add over the channels goes through shared memory, 32 values per lane and token.  4 x 2048 tokens, 2048 channels, 16 states, bfloat16:
-// 157 us the first, 419 the second, 17 the sums over blocks and pieces.  The second takes 385 instructions, 106 accesses to shared
+// 151 us the first, 419 the second, 17 the sums over blocks and pieces.  The second takes 385 instructions, 106 accesses to shared
 // memory (424 clocks of an SM quarter) and 36 exponentials (288) per token and warp and is bound by neither: with 250 registers two
-// blocks fit an SM (one of cut float32 sequences, whose shared memory is 118 KB), and two warps per quarter leave 60 % of the issue slots empty.  Four states to a lane with sums by shuffles took 525 us
-// at 3 blocks, eight states 567; limits of 168 registers spill 180 of them.
+// blocks fit an SM (one of cut float32 sequences, whose shared memory is 118 KB), and two warps per quarter leave 60 % of the issue slots
+// empty.  Four states to a lane with sums by shuffles took 525 us at 3 blocks, eight states 567; limits of 168 registers spill 180 of them.
 #include "selective_scan.cuh"
 
 namespace b200 {

@@ -51,9 +51,9 @@ struct ScanArgs {
   float *final, *dA, *dD, *ddt_bias, *dinitial;
   // the cut into pieces: tokens of a piece, pieces of a sequence (not of packed ones), of the call; blocks side by side
   int piece, pieces_per_seq, pieces, tiles;
-  float *piece_state, *piece_sum;          // [pieces][C][4 lanes], [pieces][C]: what a piece makes of zero states, its sum of deltas
-  // gradients: rows of the tensors, the states in front of every eighth token with the sums of deltas up to there, what a piece makes
-  // of a zero adjoint, partial sums: [blocks of a group][rows][groups][2][N], [pieces][C][N], [pieces][2][C]
+  float *piece_state, *piece_sum;          // [pieces][C][scan_state_slots(N)], [pieces][C]: what a piece makes of zero states, its sum of deltas
+  // gradients: rows of the tensors, the states in front of every fourth token ([scan_kept][scan_grad_slots(N) / 4][C] of four) with the sums
+  // of deltas up to there, what a piece makes of a zero adjoint, partial sums: [blocks of a group][rows][groups][2][N], [pieces][C][N], [pieces][2][C]
   long long rows;
   float *kept, *kept_sum, *piece_back, *partial_bc, *partial_a, *partial_d;
 };
