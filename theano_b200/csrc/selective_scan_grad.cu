@@ -137,8 +137,7 @@ __global__ void __launch_bounds__(kScanThreads, S * P <= 32 ? (CUT ? 3 : 4) : 1)
         for (int s = 0; s < S / 4; ++s) {
           const float4 b = bs[s];
           const Pair e0 = mul2(dd, A[2 * s]), e1 = mul2(dd, A[2 * s + 1]);
-          // none by polynomial, unlike in the forward call: the special function unit has room here (training 748 us, one pair by it 756)
-          const Pair a0 = exp2_pair(e0), a1 = exp2_pair(e1);
+          const Pair a0 = 2 * s < kPolyPairs ? exp2_poly(e0) : exp2_pair(e0), a1 = 2 * s + 1 < kPolyPairs ? exp2_poly(e1) : exp2_pair(e1);
           h[2 * s] = fma2(a0, h[2 * s], mul2(uu, Pair(b.x, b.y)));
           h[2 * s + 1] = fma2(a1, h[2 * s + 1], mul2(uu, Pair(b.z, b.w)));
           if (CUT) {
