@@ -10,7 +10,7 @@
 // zero states and of a zero adjoint).  The second walks backward: for four tokens at a time it makes their states again, in registers, and
 // runs the adjoint over them.  Both have a lane per channel with its states, so that sums over the states cost nothing; what dB and dC
 // add over the channels goes through shared memory, 32 values per lane and token.  4 x 2048 tokens, 2048 channels, 16 states, bfloat16:
-// 151 us the first, 419 the second, 17 the sums over blocks and pieces.  The second takes 385 instructions, 106 accesses to shared
+// 160 us the first, 419 the second, 17 the sums over blocks and pieces.  The second takes 385 instructions, 106 accesses to shared
 // memory (424 clocks of an SM quarter) and 36 exponentials (288) per token and warp and is bound by neither: with 250 registers two
 // blocks fit an SM (one of cut float32 sequences, whose shared memory is 118 KB), and two warps per quarter leave 60 % of the issue slots
 // empty.  Four states to a lane with sums by shuffles took 525 us at 3 blocks, eight states 567; limits of 168 registers spill 180 of them.
@@ -137,6 +137,8 @@ __global__ void __launch_bounds__(kScanThreads, S * P <= 32 ? (CUT ? 3 : 4) : 1)
         for (int s = 0; s < S / 4; ++s) {
           const float4 b = bs[s];
           const Pair e0 = mul2(dd, A[2 * s]), e1 = mul2(dd, A[2 * s + 1]);
+          // the first states by polynomial as in the forward call, for its precision: the special function unit's results near 1 are 2e-8
+          // too small on average, which slow states add up (dA of 9 x 969 tokens off by 8e-7, with it alone by 1.4e-6; 756 us, 748)
           const Pair a0 = 2 * s < kPolyPairs ? exp2_poly(e0) : exp2_pair(e0), a1 = 2 * s + 1 < kPolyPairs ? exp2_poly(e1) : exp2_pair(e1);
           h[2 * s] = fma2(a0, h[2 * s], mul2(uu, Pair(b.x, b.y)));
           h[2 * s + 1] = fma2(a1, h[2 * s + 1], mul2(uu, Pair(b.z, b.w)));
